@@ -1,0 +1,266 @@
+// Rows in 8-bit integers (int8.h): made from float rows, by themselves or behind an RMSNorm that adds to the residual stream first, and turned back; weight
+// matrices packed for the products.
+//
+//     scale = max_j |y_j| / 127          q_j = round(y_j / scale), halves to even
+//
+// in float32, the division the exact one: a value next to a border between two integers falls to the side where float32 arithmetic written down plainly has
+// it. A row of zeros has scale 0. A row that holds an infinity or a NaN has scale NaN and zeros for values, so that whatever is made of it is NaN.
+#include "int8.h"
+#include "xrt_hip.h"
+
+namespace {
+
+// Eight neighbouring elements of a row, asked for in whole pieces whatever the row's alignment (global loads need none beyond the element's).
+template <typename T> struct Eight { T e[8]; };
+template <typename T>
+__device__ __forceinline__ void load_eight(const T* row, int at, int width, float (&v)[8]) {
+    if (at + 8 <= width) {
+        Eight<T> piece;
+        __builtin_memcpy(&piece, row + at, sizeof(piece));
+#pragma unroll
+        for (int e = 0; e < 8; ++e) v[e] = to_float(piece.e[e]);
+    } else {
+#pragma unroll
+        for (int e = 0; e < 8; ++e) v[e] = at + e < width ? to_float(row[at + e]) : 0.f;
+    }
+}
+
+// The bits of |v|: as whole numbers they are ordered as the magnitudes are, infinity above all numbers and NaN above infinity.
+__device__ __forceinline__ unsigned magnitude_bits(float v) { return __builtin_bit_cast(unsigned, v) & 0x7fffffffu; }
+
+__device__ __forceinline__ unsigned wave_max_bits(unsigned v) {
+#pragma unroll
+    for (int offset = XRT_WAVE / 2; offset > 0; offset >>= 1) v = max(v, (unsigned)__shfl_xor((int)v, offset, XRT_WAVE));
+    return v;
+}
+
+// The largest of a block's magnitudes; every thread comes here and gets it. `scratch` holds 16 words that nothing else uses.
+__device__ __forceinline__ unsigned block_max_bits(unsigned v, unsigned* scratch) {
+    v = wave_max_bits(v);
+    if (threadIdx.x % XRT_WAVE == 0) scratch[threadIdx.x / XRT_WAVE] = v;
+    __syncthreads();
+    unsigned most = scratch[0];
+    for (int w = 1; w < (int)blockDim.x / XRT_WAVE; ++w) most = max(most, scratch[w]);
+    return most;
+}
+
+__device__ __forceinline__ float scale_of(unsigned most) {
+    return most >= 0x7f800000u ? __builtin_nanf("") : __builtin_bit_cast(float, most) / 127.0f;
+}
+
+// Eight values as signed bytes. (A scale too small for a normal float32 is off by up to half of itself: the quotients are clamped.)
+__device__ __forceinline__ uint2 eight_bytes(const float (&y)[8], float scale) {
+    unsigned word[2] = {0u, 0u};
+    if (scale > 0.f) {                                          // (neither zero nor NaN)
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+            const float q = fminf(fmaxf(rintf(y[e] / scale), -127.f), 127.f);
+            word[e / 4] |= ((unsigned)(int)q & 255u) << (e % 4 * 8);
+        }
+    }
+    return make_uint2(word[0], word[1]);
+}
+
+constexpr int PIECES = 4;            // pieces of eight elements that a thread keeps in registers
+constexpr int MOST_THREADS = 1024;
+
+// One workgroup a row. NORM: the row of x gets delta added (written back) and is normed before it is brought to 8 bits. A row wider than what the
+// threads keep is read again for what comes after the sums.
+template <typename TX, typename TD, typename TW, bool NORM>
+__global__ void __launch_bounds__(MOST_THREADS) int8_rows_kernel(TX* x, const TD* delta, const TW* __restrict__ weight, const int* __restrict__ rows,
+                                                                 signed char* __restrict__ values, float* __restrict__ scales, long x_stride,
+                                                                 int x_rows, int width, int stride, float eps) {
+    __shared__ float sums[32];
+    __shared__ unsigned maxima[16];
+    const long r = blockIdx.x;
+    const long source = rows ? rows[r] : r;
+    signed char* out = values + r * stride;
+    if (source < 0 || source >= x_rows) {                       // (an index that names no row)
+        for (int at = threadIdx.x * 8; at < stride; at += blockDim.x * 8) *reinterpret_cast<uint2*>(out + at) = make_uint2(0u, 0u);
+        if (threadIdx.x == 0) scales[r] = __builtin_nanf("");
+        return;
+    }
+    TX* row = x + source * x_stride;
+    const TD* add = NORM && delta ? delta + source * width : nullptr;
+    const int step = blockDim.x * 8, first = threadIdx.x * 8;
+    float kept[PIECES][8];
+    float inv_rms = 1.f;
+#pragma unroll
+    for (int i = 0; i < PIECES; ++i) load_eight(row, first + i * step, width, kept[i]);
+    if constexpr (NORM) {
+        auto added = [&](int at, float (&v)[8]) {
+            if (!add || at >= width) return;
+            float d[8];
+            load_eight(add, at, width, d);
+#pragma unroll
+            for (int e = 0; e < 8; ++e) v[e] += d[e];
+            if (at + 8 <= width) {
+                Eight<TX> piece;
+#pragma unroll
+                for (int e = 0; e < 8; ++e) piece.e[e] = from_float<TX>(v[e]);
+                __builtin_memcpy(row + at, &piece, sizeof(piece));
+            } else {
+                for (int e = 0; at + e < width; ++e) row[at + e] = from_float<TX>(v[e]);
+            }
+        };
+        float sum = 0.f;
+#pragma unroll
+        for (int i = 0; i < PIECES; ++i) {
+            added(first + i * step, kept[i]);
+#pragma unroll
+            for (int e = 0; e < 8; ++e) sum = fmaf(kept[i][e], kept[i][e], sum);
+        }
+        for (int at = first + PIECES * step; at < width; at += step) {
+            float v[8];
+            load_eight(row, at, width, v);
+            added(at, v);
+#pragma unroll
+            for (int e = 0; e < 8; ++e) sum = fmaf(v[e], v[e], sum);
+        }
+        inv_rms = 1.0f / sqrtf(block_sum(sum, sums) / (float)width + eps);
+    }
+    // what is brought to 8 bits, of what the row holds (a thread reads again only what it wrote itself)
+    auto finished = [&](int at, float (&v)[8]) {
+        if constexpr (NORM) {
+            float gain[8];
+            load_eight(weight, at, width, gain);
+#pragma unroll
+            for (int e = 0; e < 8; ++e) v[e] = v[e] * inv_rms * gain[e];
+        }
+    };
+    unsigned most = 0u;
+#pragma unroll
+    for (int i = 0; i < PIECES; ++i) {
+        finished(first + i * step, kept[i]);
+#pragma unroll
+        for (int e = 0; e < 8; ++e) most = max(most, magnitude_bits(kept[i][e]));
+    }
+    for (int at = first + PIECES * step; at < width; at += step) {
+        float v[8];
+        load_eight(row, at, width, v);
+        finished(at, v);
+#pragma unroll
+        for (int e = 0; e < 8; ++e) most = max(most, magnitude_bits(v[e]));
+    }
+    const float scale = scale_of(block_max_bits(most, maxima));
+#pragma unroll
+    for (int i = 0; i < PIECES; ++i)
+        if (first + i * step < stride) *reinterpret_cast<uint2*>(out + first + i * step) = eight_bytes(kept[i], scale);
+    for (int at = first + PIECES * step; at < stride; at += step) {
+        float v[8];
+        load_eight(row, at, width, v);
+        finished(at, v);
+        *reinterpret_cast<uint2*>(out + at) = eight_bytes(v, scale);
+    }
+    if (threadIdx.x == 0) scales[r] = scale;
+}
+
+// out[m][j] = values[m][j] * scales[m]: a thread eight neighbouring columns
+template <typename TO>
+__global__ void __launch_bounds__(256) int8_values_kernel(const signed char* __restrict__ values, const float* __restrict__ scales, TO* __restrict__ out,
+                                                          int rows, int width, int stride) {
+    const long pieces = (width + 7) / 8, id = (long)blockIdx.x * blockDim.x + threadIdx.x;
+    const long r = id / pieces;
+    if (r >= rows) return;
+    const int at = (int)(id % pieces) * 8;
+    const uint2 bytes = *reinterpret_cast<const uint2*>(values + r * stride + at);
+    const float scale = scales[r];
+    TO* row = out + r * width;
+    Eight<TO> piece;
+#pragma unroll
+    for (int e = 0; e < 8; ++e) piece.e[e] = from_float<TO>((float)(int)(signed char)((e < 4 ? bytes.x : bytes.y) >> (e % 4 * 8)) * scale);
+    if (at + 8 <= width) __builtin_memcpy(row + at, &piece, sizeof(piece));
+    else
+        for (int e = 0; at + e < width; ++e) row[at + e] = piece.e[e];
+}
+
+// A thread a 16-byte piece of the packed matrix; the threads of the first tile of a group see to its scales.
+__global__ void __launch_bounds__(256) int8_pack_kernel(const signed char* __restrict__ values, const float* __restrict__ scales,
+                                                        signed char* __restrict__ packed, float* __restrict__ packed_scales, int n, int stride,
+                                                        long pieces, int gated) {
+    const long id = (long)blockIdx.x * blockDim.x + threadIdx.x;
+    if (id >= pieces) return;
+    const int lane = (int)(id % XRT_WAVE), tiles = stride / 64;
+    const long tile = id / XRT_WAVE, group = tile / tiles;
+    const int within = lane % 16;
+    long row = gated ? group * 8 + within % 8 : group * 16 + within;
+    const bool there = row < n;
+    if (gated && within >= 8) row += n;
+    const long column = tile % tiles * 64 + lane / 16 * 16;
+    uint4 piece = make_uint4(0u, 0u, 0u, 0u);
+    if (there) piece = *reinterpret_cast<const uint4*>(values + row * stride + column);
+    *reinterpret_cast<uint4*>(packed + id * 16) = piece;
+    if (tile % tiles == 0 && lane < 16) packed_scales[group * 16 + within] = there ? scales[row] : 0.f;
+}
+
+// Threads of a row's workgroup: two pieces of eight a thread, or what keeps the row in registers, if it can be.
+int threads_for(int stride) {
+    const int pieces = stride / 8;
+    const int wanted = pieces <= 2 * MOST_THREADS ? (pieces + 1) / 2 : MOST_THREADS;
+    return whole_wavefronts(wanted);
+}
+
+}  // namespace
+
+extern "C" long xrt_int8_stride(int k) { return int8_stride(k); }
+extern "C" long xrt_int8_packed_rows(int n, int gated) { return int8_groups(n, gated != 0) * 16; }
+
+extern "C" int xrt_quantize_int8(const void* x, int dtype, long x_stride, void* values, float* scales, int rows, int k, void* stream) {
+    XRT_REQUIRE(rows >= 0 && k > 0 && k <= XRT_INT8_MOST_K && (rows == 0 || (x && values && scales)), "quantize_int8: bad operands rows=%d k=%d", rows, k);
+    XRT_REQUIRE(dtype == XRT_F32 || dtype == XRT_BF16, "quantize_int8: unknown dtype %d", dtype);
+    XRT_REQUIRE(x_stride >= k, "quantize_int8: rows of %d elements %ld apart", k, x_stride);
+    if (rows == 0) return 0;
+    const int stride = (int)int8_stride(k), threads = threads_for(stride);
+    hipStream_t s = (hipStream_t)stream;
+    if (dtype == XRT_F32)
+        int8_rows_kernel<float, float, float, false><<<rows, threads, 0, s>>>((float*)x, nullptr, nullptr, nullptr, (signed char*)values, scales, x_stride, rows, k, stride, 0.f);
+    else
+        int8_rows_kernel<bf16, float, float, false><<<rows, threads, 0, s>>>((bf16*)x, nullptr, nullptr, nullptr, (signed char*)values, scales, x_stride, rows, k, stride, 0.f);
+    XRT_LAUNCH_CHECK("quantize_int8");
+    return 0;
+}
+
+extern "C" int xrt_rmsnorm_int8(float* x, const void* delta, int delta_dtype, const void* weight, int weight_dtype, float eps, void* values, float* scales,
+                                const int* rows, int n_rows, int x_rows, int hidden, void* stream) {
+    XRT_REQUIRE(n_rows >= 0 && x_rows >= 0 && hidden > 0 && hidden <= XRT_INT8_MOST_K && (n_rows == 0 || (x && weight && values && scales)),
+                "rmsnorm_int8: bad operands rows=%d hidden=%d", n_rows, hidden);
+    XRT_REQUIRE((weight_dtype == XRT_F32 || weight_dtype == XRT_BF16) && (!delta || delta_dtype == XRT_F32 || delta_dtype == XRT_BF16),
+                "rmsnorm_int8: unknown dtype weight=%d delta=%d", weight_dtype, delta_dtype);
+    XRT_REQUIRE(!delta || !rows, "rmsnorm_int8: chosen rows of x cannot be added to (one might be chosen twice)");
+    XRT_REQUIRE(rows || n_rows == x_rows, "rmsnorm_int8: %d rows of results for %d rows of x", n_rows, x_rows);
+    if (n_rows == 0) return 0;
+    const int stride = (int)int8_stride(hidden), threads = threads_for(stride);
+    hipStream_t s = (hipStream_t)stream;
+#define XRT_NORM8(TD, TW) int8_rows_kernel<float, TD, TW, true><<<n_rows, threads, 0, s>>>(x, (const TD*)delta, (const TW*)weight, rows, (signed char*)values, scales, hidden, x_rows, hidden, stride, eps)
+    if (delta_dtype == XRT_BF16 && weight_dtype == XRT_BF16) XRT_NORM8(bf16, bf16);
+    else if (delta_dtype == XRT_BF16) XRT_NORM8(bf16, float);
+    else if (weight_dtype == XRT_BF16) XRT_NORM8(float, bf16);
+    else XRT_NORM8(float, float);
+#undef XRT_NORM8
+    XRT_LAUNCH_CHECK("rmsnorm_int8");
+    return 0;
+}
+
+extern "C" int xrt_dequantize_int8(const void* values, const float* scales, void* out, int out_dtype, int rows, int k, void* stream) {
+    XRT_REQUIRE(rows >= 0 && k > 0 && k <= XRT_INT8_MOST_K && (rows == 0 || (values && scales && out)), "dequantize_int8: bad operands rows=%d k=%d", rows, k);
+    XRT_REQUIRE(out_dtype == XRT_F32 || out_dtype == XRT_BF16, "dequantize_int8: unknown dtype %d", out_dtype);
+    if (rows == 0) return 0;
+    const long blocks = ((long)rows * ((k + 7) / 8) + 255) / 256;
+    XRT_REQUIRE(blocks < (1L << 31), "dequantize_int8: too many elements");
+    hipStream_t s = (hipStream_t)stream;
+    if (out_dtype == XRT_F32) int8_values_kernel<float><<<(unsigned)blocks, 256, 0, s>>>((const signed char*)values, scales, (float*)out, rows, k, (int)int8_stride(k));
+    else int8_values_kernel<bf16><<<(unsigned)blocks, 256, 0, s>>>((const signed char*)values, scales, (bf16*)out, rows, k, (int)int8_stride(k));
+    XRT_LAUNCH_CHECK("dequantize_int8");
+    return 0;
+}
+
+extern "C" int xrt_pack_int8(const void* values, const float* scales, void* packed, float* packed_scales, int n, int k, int gated, void* stream) {
+    XRT_REQUIRE(values && scales && packed && packed_scales && n > 0 && k > 0 && k <= XRT_INT8_MOST_K, "pack_int8: bad operands n=%d k=%d", n, k);
+    const long pieces = int8_groups(n, gated != 0) * int8_stride(k);             // 16 rows of stride bytes, 16 bytes a piece
+    const long blocks = (pieces + 255) / 256;
+    XRT_REQUIRE(blocks < (1L << 31), "pack_int8: too many elements");
+    int8_pack_kernel<<<(unsigned)blocks, 256, 0, (hipStream_t)stream>>>((const signed char*)values, scales, (signed char*)packed, packed_scales, n,
+                                                                        (int)int8_stride(k), pieces, gated != 0);
+    XRT_LAUNCH_CHECK("pack_int8");
+    return 0;
+}

@@ -107,6 +107,30 @@ long xrt_linear_static_floats(void);       // XRT_LINEAR_STATIC_FLOATS, for call
 int xrt_linear_static(const void* a, const void* w, int dtype, void* out, int out_dtype, int M, int N, int K,
                       int mode, void* stream);
 
+// ---- rows and weight matrices in 8-bit integers with scales (csrc/int8.h says how they lie) ----
+// Row m of k columns is values[m][0 .. xrt_int8_stride(k)), signed bytes with zeros from column k on, times scales[m] (float32). values start at a
+// multiple of 16 bytes. k is at most XRT_INT8_K_LIMIT, so that sums of products are exact in 32 bits.
+#define XRT_INT8_K_LIMIT 131071
+long xrt_int8_stride(int k);
+// scales[m] = max |x[m]| / 127, values = x / scale rounded to the nearest integer, halves to even; x (float32 or bfloat16) has its rows x_stride
+// elements apart. A row of zeros: scale 0; one with an infinity or a NaN: scale NaN and zeros.
+int xrt_quantize_int8(const void* x, int dtype, long x_stride, void* values, float* scales, int rows, int k, void* stream);
+// x[m] += delta[m] (delta may be null), then the rows rmsnorm(x[rows ? rows[r] : r]) * weight likewise; delta and rows not both. x has x_rows rows; an
+// index that is none of them gives zeros with scale NaN.
+int xrt_rmsnorm_int8(float* x, const void* delta, int delta_dtype, const void* weight, int weight_dtype, float eps, void* values, float* scales,
+                     const int* rows, int n_rows, int x_rows, int hidden, void* stream);
+// out[m][j] = values[m][j] * scales[m]
+int xrt_dequantize_int8(const void* values, const float* scales, void* out, int out_dtype, int rows, int k, void* stream);
+// A matrix of n rows (gated: 2 n, gate rows then up rows) packed for xrt_linear_int8: xrt_int8_packed_rows(n, gated) rows of xrt_int8_stride(k) bytes,
+// and as many scales.
+long xrt_int8_packed_rows(int n, int gated);
+int xrt_pack_int8(const void* values, const float* scales, void* packed, float* packed_scales, int n, int k, int gated, void* stream);
+// out[m][n] (+)= (sum_k a[m][k] * w[n][k]) * a_scales[m] * w_scales[n], modes as xrt_linear has them, w packed (mode 2: as a gated matrix); the sum is exact,
+// so the result of a row does not depend on the others. xrt_linear_int8_workspace: the bytes that a product split along k needs (0: none).
+int xrt_linear_int8(const void* a, const float* a_scales, const void* w, const float* w_scales, void* out, int out_dtype, int M, int N, int K,
+                    int mode, void* workspace, long workspace_bytes, void* stream);
+long xrt_linear_int8_workspace(int M, int N, int K, int mode);
+
 // An RMSNorm between two products, x += a w^T; y = rmsnorm(x) * gain; z = y v^T, without a kernel of
 // its own. The first product (mode 1) also writes scaled_out[m, n] = bfloat16(x[m, n] * gain[n]) and
 // squares_out[t * XRT_SQUARES_STRIDE + m], the sum of x[m, n]^2 over the columns n of tile t (xrt_linear_norm_tiles of them, 16 columns or fewer each). The

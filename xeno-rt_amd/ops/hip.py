@@ -109,6 +109,46 @@ def _matrix(w):
     return w, None
 
 
+INT8_STEP = 128             # columns that a row of 8-bit values is filled up to whole numbers of (XRT_INT8_STEP of the library)
+INT8_MOST_K = 131071        # columns of which a sum of products still fits 32 bits (XRT_INT8_MOST_K)
+
+
+class Int8Rows:
+    """Rows in 8-bit integers: row m stands for values[m, :k] * scales[m]. values is int8 [rows, k filled up to a multiple of INT8_STEP], with zeros
+    behind the k columns; scales float32 [rows]. `int8_rows` makes an empty one; `quantize_int8` and `rmsnorm_int8` fill it, `linear_int8` and
+    `linear_glu_int8` multiply it. Whoever fills one in another way keeps the zeros."""
+
+    __slots__ = ("values", "scales", "k")
+
+    def __init__(self, values: torch.Tensor, scales: torch.Tensor, k: int):
+        self.values, self.scales, self.k = values, scales, int(k)
+
+    @property
+    def shape(self):
+        return (self.values.shape[0], self.k)
+
+    @property
+    def device(self):
+        return self.values.device
+
+
+class Int8Matrix:
+    """A weight matrix [rows, k] in 8-bit integers with a scale for each row (output channel), in the tiles in which the products take it
+    (csrc/int8.h). gated: [gate rows | up rows], for `linear_glu_int8`. Made by `pack_int8`."""
+
+    __slots__ = ("data", "scales", "shape", "gated")
+
+    def __init__(self, data: torch.Tensor, scales: torch.Tensor, rows: int, k: int, gated: bool):
+        self.data, self.scales, self.shape, self.gated = data, scales, (rows, k), gated
+
+    @property
+    def device(self):
+        return self.data.device
+
+    def dim(self) -> int:
+        return 2
+
+
 class _QkvFinish(ctypes.Structure):
     _fields_ = [("q_norm", ctypes.c_void_p), ("k_norm", ctypes.c_void_p), ("norm_dtype", ctypes.c_int),
                 ("norm_eps", ctypes.c_float), ("rope_dim", ctypes.c_int), ("rope_table", ctypes.c_void_p),
@@ -240,7 +280,8 @@ class HipOps:
                      "xrt_experts_sort", "xrt_gather_rows", "xrt_linear_groups", "xrt_linear_groups_accepts", "xrt_experts_combine",
                      "xrt_linear_groups_tile_rows", "xrt_linear_groups_parts", "xrt_streams_open", "xrt_streams_read", "xrt_streams_write",
                      "xrt_latent_complete", "xrt_latent_queries", "xrt_linear_heads", "xrt_causal_softmax", "xrt_transpose", "xrt_attention_latent",
-                     "xrt_attention_latent_accepts", "xrt_attention_latent_prompts", "xrt_latent_prepare", "xrt_glu_experts", "xrt_embed_normed", "xrt_rmsnorm_two", "xrt_replace_rows"):
+                     "xrt_attention_latent_accepts", "xrt_attention_latent_prompts", "xrt_latent_prepare", "xrt_glu_experts", "xrt_embed_normed", "xrt_rmsnorm_two", "xrt_replace_rows",
+                     "xrt_quantize_int8", "xrt_rmsnorm_int8", "xrt_dequantize_int8", "xrt_pack_int8", "xrt_linear_int8"):
             getattr(self.lib, name).restype = ctypes.c_int
         from ..cache.allocator import BLOCK_TOKENS
         if int(self.lib.xrt_block_tokens()) != BLOCK_TOKENS:
@@ -257,6 +298,7 @@ class HipOps:
         self.lib.xrt_selective_scan_workspace.restype = ctypes.c_long
         self.lib.xrt_experts_sort_room.restype = ctypes.c_long
         self.lib.xrt_attention_latent_workspace.restype = ctypes.c_long
+        self.lib.xrt_linear_int8_workspace.restype = ctypes.c_long
 
     # -- helpers -------------------------------------------------------------
     def _check(self, status: int) -> None:
@@ -530,6 +572,129 @@ class HipOps:
         if activation not in ACTIVATIONS:
             raise KernelError(f"linear_glu: activation must be one of {sorted(ACTIVATIONS)}, found {activation!r}")
         self._linear(a, w_gate_up, out, 2 | (ACTIVATIONS[activation] << 8), w_gate_up.shape[0] // 2)
+
+    # -- rows and weights in 8-bit integers --------------------------------------
+    @staticmethod
+    def _on_current_device(tensor) -> None:
+        """The kernels start on the current device: tensors of another one are refused."""
+        if tensor.get_device() != torch.cuda.current_device():
+            raise KernelError(f"the tensors are on {tensor.device}, the current device is cuda:{torch.cuda.current_device()}")
+
+    def _require_int8(self, rows, what: str, shape, like=None) -> None:
+        if not isinstance(rows, Int8Rows):
+            raise KernelError(f"{what}: expected Int8Rows")
+        if rows.shape != tuple(shape):
+            raise KernelError(f"{what}: rows of shape {rows.shape}, expected {tuple(shape)}")
+        count, k = shape
+        if not 0 < k <= INT8_MOST_K:
+            raise KernelError(f"{what}: rows of {k} columns, expected 1 to {INT8_MOST_K}")
+        self._require(rows.values, f"{what} values", torch.int8, (count, (k + INT8_STEP - 1) // INT8_STEP * INT8_STEP), like)
+        self._require(rows.scales, f"{what} scales", torch.float32, (count,), rows.values)
+        if rows.values.data_ptr() % 16 != 0:                    # (they are read sixteen bytes at a time)
+            raise KernelError(f"{what}: values must start at a multiple of 16 bytes")
+
+    def int8_rows(self, rows: int, k: int, device) -> Int8Rows:
+        """Room for `rows` rows of k columns in 8-bit integers; what it holds is not defined."""
+        if rows < 0 or not 0 < k <= INT8_MOST_K:
+            raise KernelError(f"int8_rows: {rows} rows of {k} columns; up to {INT8_MOST_K} columns are possible")
+        return Int8Rows(self._empty((rows, (k + INT8_STEP - 1) // INT8_STEP * INT8_STEP), torch.int8, device),
+                        self._empty((rows,), torch.float32, device), k)
+
+    def quantize_int8(self, x, out: Int8Rows):
+        """out = the rows of x (float32 or bfloat16, some columns of a wider matrix will do) in 8-bit integers: scales[m] = max |x[m]| / 127, values =
+        x / scale rounded to the nearest integer, halves to even. A row of zeros has scale 0; one that holds an infinity or a NaN scale NaN and zeros."""
+        stride = self._rows(x, "quantize_int8 x")
+        code = _code(x)
+        self._require_int8(out, "quantize_int8 out", x.shape, x)
+        self._on_current_device(x)
+        self._check(self.lib.xrt_quantize_int8(_ptr(x), code, ctypes.c_long(stride), _ptr(out.values), _ptr(out.scales), x.shape[0], x.shape[1],
+                                               self._stream(x)))
+
+    def rmsnorm_int8(self, x, weight, eps, out: Int8Rows, delta=None, rows=None):
+        """x += delta in place, if given (float32 or bfloat16, shaped like x), then out = the rows x / sqrt(mean(x^2) + eps) * weight as `quantize_int8`
+        would make them of float32. x is float32. rows: the rows of x that are wanted, as in `rmsnorm` (not together with delta); one that x does not
+        have gives zeros with scale NaN."""
+        self._require(x, "rmsnorm_int8 x", torch.float32)
+        if x.dim() != 2:
+            raise KernelError("rmsnorm_int8 x: expected [rows, hidden]")
+        x_rows, hidden = x.shape
+        self._require(weight, "rmsnorm_int8 weight", None, (hidden,), x)
+        count = x_rows
+        if rows is not None:
+            if delta is not None:
+                raise KernelError("rmsnorm_int8: chosen rows of x cannot be added to (one might be chosen twice)")
+            if not isinstance(rows, torch.Tensor) or rows.dim() != 1:
+                raise KernelError("rmsnorm_int8 rows: expected a list of rows on the GPU")
+            count = rows.shape[0]
+            self._require(rows, "rmsnorm_int8 rows", torch.int32, (count,), x)
+        if delta is not None:
+            self._require(delta, "rmsnorm_int8 delta", None, (x_rows, hidden), x)
+        self._require_int8(out, "rmsnorm_int8 out", (count, hidden), x)
+        self._on_current_device(x)
+        self._check(self.lib.xrt_rmsnorm_int8(_ptr(x), _ptr(delta), 0 if delta is None else _code(delta), _ptr(weight), _code(weight), ctypes.c_float(eps),
+                                              _ptr(out.values), _ptr(out.scales), _ptr(rows), count, x_rows, hidden, self._stream(x)))
+
+    def dequantize_int8(self, rows: Int8Rows, out):
+        """out[m, j] = values[m, j] * scales[m] (float32 or bfloat16)."""
+        self._require_int8(rows, "dequantize_int8 rows", rows.shape)
+        self._require(out, "dequantize_int8 out", None, rows.shape, rows.values)
+        self._on_current_device(out)
+        self._check(self.lib.xrt_dequantize_int8(_ptr(rows.values), _ptr(rows.scales), _ptr(out), _code(out), rows.shape[0], rows.k, self._stream(out)))
+
+    def pack_int8(self, w, gated: bool = False) -> Int8Matrix:
+        """The weight matrix w [rows, k] for `linear_int8`, or gated ([gate rows | up rows]) for `linear_glu_int8`: Int8Rows, or a float matrix, whose
+        rows (output channels) are then brought to 8 bits as `quantize_int8` does it."""
+        if not isinstance(w, Int8Rows):
+            if not isinstance(w, torch.Tensor) or w.dim() != 2 or 0 in w.shape:
+                raise KernelError("pack_int8: w must be [rows, k]")
+            as_rows = self.int8_rows(w.shape[0], w.shape[1], w.device)
+            self.quantize_int8(w, as_rows)
+            w = as_rows
+        rows, k = w.shape
+        if rows < 1 or (gated and rows % 2 != 0):
+            raise KernelError(f"pack_int8: {rows} rows; a gated matrix has gate rows followed by as many up rows")
+        self._require_int8(w, "pack_int8 w", w.shape)
+        self._on_current_device(w.values)
+        n = rows // 2 if gated else rows
+        packed_rows = (n + 7) // 8 * 16 if gated else (n + 15) // 16 * 16
+        data = torch.empty(packed_rows, w.values.shape[1], dtype=torch.int8, device=w.device)
+        scales = torch.empty(packed_rows, dtype=torch.float32, device=w.device)
+        self._check(self.lib.xrt_pack_int8(_ptr(w.values), _ptr(w.scales), _ptr(data), _ptr(scales), n, k, int(gated), self._stream(data)))
+        return Int8Matrix(data, scales, rows, k, bool(gated))
+
+    def _linear_int8(self, a, w, out, mode, n):
+        if not isinstance(w, Int8Matrix):
+            raise KernelError("linear_int8 w: expected an Int8Matrix")
+        rows, k = w.shape
+        m = a.shape[0]
+        self._require_int8(a, "linear_int8 a", (m, k), w.data)
+        self._require(out, "linear_int8 out", None, (m, n), w.data)
+        if mode == 1 and out.dtype != torch.float32:
+            raise KernelError(f"linear_int8 out: added to in {out.dtype}, expected float32")
+        self._on_current_device(out)
+        need = int(self.lib.xrt_linear_int8_workspace(m, n, k, mode))
+        workspace = self._empty(need // 4, torch.int32, out.device) if need > 0 else None
+        self._check(self.lib.xrt_linear_int8(_ptr(a.values), _ptr(a.scales), _ptr(w.data), _ptr(w.scales), _ptr(out), _code(out), m, n, k, mode,
+                                             _ptr(workspace), ctypes.c_long(need), self._stream(out)))
+
+    def linear_int8(self, a: Int8Rows, w: Int8Matrix, out, accumulate=False):
+        """out[m, n] (+)= (sum over j of a[m, j] w[n, j], exact) * a.scales[m] * w.scales[n], in float32; out is float32 or bfloat16, float32 if it is
+        added to. A row's result has the same bits whatever the other rows are."""
+        if isinstance(w, Int8Matrix) and w.gated:
+            raise KernelError("linear_int8 w: packed for linear_glu_int8")
+        if not isinstance(a, Int8Rows):
+            raise KernelError("linear_int8 a: expected Int8Rows")
+        self._linear_int8(a, w, out, 1 if accumulate else 0, w.shape[0])
+
+    def linear_glu_int8(self, a: Int8Rows, w_gate_up: Int8Matrix, out, activation: str = "silu"):
+        """out = act(gate) * up of the two products with w_gate_up = [gate rows | up rows], each as `linear_int8` makes it."""
+        if isinstance(w_gate_up, Int8Matrix) and not w_gate_up.gated:
+            raise KernelError("linear_glu_int8 w: packed for linear_int8")
+        if not isinstance(a, Int8Rows):
+            raise KernelError("linear_glu_int8 a: expected Int8Rows")
+        if activation not in ACTIVATIONS:
+            raise KernelError(f"linear_glu_int8: activation must be one of {sorted(ACTIVATIONS)}, found {activation!r}")
+        self._linear_int8(a, w_gate_up, out, 2 | (ACTIVATIONS[activation] << 8), w_gate_up.shape[0] // 2)
 
     def _prepare_arguments(self, qkv, n_heads, n_kv_heads, head_dim, positions, slots, q_norm, k_norm, norm_eps,
                            rope_theta, rope_dim, rope_scale, kv, longest_run):
