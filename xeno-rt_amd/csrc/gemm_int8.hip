@@ -4,93 +4,588 @@
 //
 // The sum is exact: whole numbers of 32 bits (k is limited so that it cannot overflow). Every kernel here therefore gives the same bits for a row of a,
 // however many other rows there are and however k is cut. It is rounded to float32 once, then multiplied by the row's and by the channel's scale.
+//
+// v_mfma_i32_16x16x64_i8 takes w as its A operand and a as its B operand: lane (r, c) = (lane % 16, lane / 16) holds columns 16 c .. 16 c + 15 of packed row
+// r of w and of row r of a, and gets the sums of row r of a with packed rows 4 c .. 4 c + 3 of w. A "block" below is such a 16 x 16 piece of the result.
+//
+// Up to 64 rows the product is bound by reading w, and gemm_int8_few_kernel streams it through registers. More rows go through tiles in LDS
+// (gemm_int8_large_kernel). Where there are too few workgroups for the chip, k is cut into parts whose sums, as the lanes hold them, go to a workspace;
+// int8_finish_kernel adds them and does the rest.
+#include <type_traits>
 #include "int8.h"
 #include "activation.h"
-#include "xrt_hip.h"
+#include "large_tiles.h"
 
 namespace {
 
 typedef int int4v __attribute__((ext_vector_type(4)));
 enum { MODE_STORE = 0, MODE_ACCUMULATE = 1, MODE_GATED = 2 };
 
-// One value of the result; `before` is what out holds.
 __device__ __forceinline__ float scaled(int sum, float a_scale, float w_scale) { return (float)sum * a_scale * w_scale; }
 
-// The simple one: a wavefront has 16 packed rows of w and 64 rows of a, and loads its operands from global memory.
+// What a product writes, and what the sums are multiplied by.
+template <typename TO>
+struct Result {
+    const float* a_scales;
+    const float* w_scales;      // in the order of the packed rows
+    TO* out;                    // [M][N]
+    int M, N, activation;
+};
+
+// Writes the block of rows m0 .. m0 + 15 of a and group `group` of w.
 template <int MODE, typename TO>
-__global__ void __launch_bounds__(256) gemm_int8_kernel(const signed char* __restrict__ a, const float* __restrict__ a_scales,
-                                                        const signed char* __restrict__ w, const float* __restrict__ w_scales, TO* __restrict__ out,
-                                                        int M, int N, int stride, int groups, int activation) {
-    const int lane = threadIdx.x % XRT_WAVE, wave = threadIdx.x / XRT_WAVE;
-    const int group = blockIdx.x * 4 + wave;
-    if (group >= groups) return;
-    const int r = lane % 16, c = lane / 16;
-    const long m0 = (long)blockIdx.y * 64;
-    const signed char* w_at = w + (long)group * 16 * stride + lane * 16;
-    const signed char* a_at[4];
-    int4v sum[4];
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-        const long m = m0 + i * 16 + r;
-        a_at[i] = a + (m < M ? m : (long)M - 1) * stride + c * 16;
-        sum[i] = int4v{0, 0, 0, 0};
-    }
-    for (int k = 0; k < stride; k += 64) {
-        const int4v wk = *reinterpret_cast<const int4v*>(w_at + (long)k * 16);
-#pragma unroll
-        for (int i = 0; i < 4; ++i) sum[i] = __builtin_amdgcn_mfma_i32_16x16x64_i8(wk, *reinterpret_cast<const int4v*>(a_at[i] + k), sum[i], 0, 0, 0);
-    }
-    // element e of sum[i]: row m0 + i * 16 + r of a, packed row group * 16 + c * 4 + e of w
-    float w_scale[4];
-#pragma unroll
-    for (int e = 0; e < 4; ++e) w_scale[e] = w_scales[group * 16 + c * 4 + e];
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-        const long m = m0 + i * 16 + r;
-        const float a_scale = a_scales[m < M ? m : (long)M - 1];
+__device__ __forceinline__ void finish_block(const int4v sum, long m0, long group, const Result<TO>& to) {
+    const int lane = threadIdx.x % XRT_WAVE, r = lane % 16, c = lane / 16;
+    const long m = m0 + r;
+    const float a_scale = to.a_scales[m < to.M ? m : (long)to.M - 1];
+    const float4 w_scale = *reinterpret_cast<const float4*>(to.w_scales + group * 16 + c * 4);
+    float value[4] = {scaled(sum[0], a_scale, w_scale.x), scaled(sum[1], a_scale, w_scale.y), scaled(sum[2], a_scale, w_scale.z), scaled(sum[3], a_scale, w_scale.w)};
+    long n = group * 16 + c * 4;
+    bool mine = m < to.M;
+    if constexpr (MODE == MODE_GATED) {
+        // lanes c = 0, 1 hold the gate sums of outputs 8 group + 4 c + e, lanes c = 2, 3 the up sums of the same
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
-            float value = scaled(sum[i][e], a_scale, w_scale[e]);
-            long n = (long)group * 16 + c * 4 + e;
-            bool mine = m < M;
-            if constexpr (MODE == MODE_GATED) {
-                const float up = of_other_half(value);
-                value = gate_activation<sizeof(TO) == 2>(value, activation) * up;
-                n = (long)group * 8 + c * 4 + e;
-                mine = mine && c < 2;
+            const float up = of_other_half(value[e]);
+            value[e] = gate_activation<sizeof(TO) == 2>(value[e], to.activation) * up;
+        }
+        n = group * 8 + c * 4;
+        mine = mine && c < 2;
+    }
+    if (!mine || n >= to.N) return;
+    const bool wide = to.N % 4 == 0 && (uintptr_t)to.out % 16 == 0;
+    if constexpr (MODE == MODE_ACCUMULATE) {
+        float before[4];
+        load_four<TO>(to.out, m, n, to.M, to.N, before, wide);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) value[e] = before[e] + value[e];
+    }
+    store_four<TO>(to.out, m, n, to.M, to.N, value, wide);
+}
+
+// Adds the parts of every block, one wavefront a block: sums[part][16 rows of a][group][lane].
+template <int MODE, typename TO>
+__global__ void __launch_bounds__(256) int8_finish_kernel(const int4v* __restrict__ sums, int parts, int groups, long blocks, const Result<TO> to) {
+    const long block = (long)blockIdx.x * 4 + threadIdx.x / XRT_WAVE;
+    if (block >= blocks) return;
+    const int4v* at = sums + block * XRT_WAVE + threadIdx.x % XRT_WAVE;
+    int4v sum = at[0];
+#pragma unroll 8
+    for (int p = 1; p < parts; ++p) sum += at[p * blocks * XRT_WAVE];
+    finish_block<MODE, TO>(sum, block / groups * 16, block % groups, to);
+}
+
+// ---- up to 64 rows ----------------------------------------------------------------------------------------------------------------------------------------
+
+constexpr int WAVES = 8;
+
+// MT: blocks of 16 rows of a (all of them); G: groups of 16 packed rows of w a workgroup. Its wavefronts share out k, each with a run of its own, and add
+// their sums through LDS. Nothing is read twice by a workgroup, so a's rows come from L2 as often as there are workgroups: with G groups a workgroup reads
+// MT / G times as much of a as of w. PARTS: k is cut among blockIdx.y.
+template <int MT, int G, int MODE, typename TO, bool PARTS>
+__global__ void __launch_bounds__(WAVES * XRT_WAVE, MT * G <= 2 ? 4 : 2) gemm_int8_few_kernel(const signed char* __restrict__ a, const signed char* __restrict__ w,
+                                                                                          int4v* __restrict__ sums, int M, int stride, int groups, int parts,
+                                                                                          const Result<TO> to) {
+    constexpr int AT_ONCE = G * MT < 8 ? G * MT : 8;            // blocks whose sums lie in LDS at one time
+    __shared__ int4v shared[WAVES][AT_ONCE][XRT_WAVE];
+    const int lane = threadIdx.x % XRT_WAVE, wave = __builtin_amdgcn_readfirstlane(threadIdx.x / XRT_WAVE);
+    const int r = lane % 16, c = lane / 16;
+    const int first_group = blockIdx.x * G;
+
+    // units of 128 columns, dealt evenly to the parts and within a part to the wavefronts
+    const int units = stride / XRT_INT8_STEP;
+    const int part = PARTS ? blockIdx.y : 0;
+    const int begin = PARTS ? (int)((long)units * part / parts) : 0, end = PARTS ? (int)((long)units * (part + 1) / parts) : units;
+    const int first = begin + (end - begin) * wave / WAVES, count = begin + (end - begin) * (wave + 1) / WAVES - first;
+
+    const signed char* w_at[G];
+    const signed char* a_at[MT];
+#pragma unroll
+    for (int g = 0; g < G; ++g) w_at[g] = w + (long)min(first_group + g, groups - 1) * 16 * stride + (long)first * 2048 + lane * 16;       // groups beyond the matrix: the last one again
+#pragma unroll
+    for (int i = 0; i < MT; ++i) a_at[i] = a + (long)min(i * 16 + r, M - 1) * stride + (long)first * 128 + c * 16;                         // rows likewise
+
+    struct Unit { int4v w[G][2], a[MT][2]; };
+    auto load = [&](Unit& unit, int u) {
+#pragma unroll
+        for (int i = 0; i < MT; ++i)
+#pragma unroll
+            for (int j = 0; j < 2; ++j) unit.a[i][j] = *reinterpret_cast<const int4v*>(a_at[i] + (long)u * 128 + j * 64);
+#pragma unroll
+        for (int g = 0; g < G; ++g)
+#pragma unroll
+            for (int j = 0; j < 2; ++j) unit.w[g][j] = __builtin_nontemporal_load(reinterpret_cast<const int4v*>(w_at[g] + (long)u * 2048 + j * 1024));
+    };
+    int4v acc[G][MT];
+#pragma unroll
+    for (int g = 0; g < G; ++g)
+#pragma unroll
+        for (int i = 0; i < MT; ++i) acc[g][i] = int4v{0, 0, 0, 0};
+    auto multiply = [&](const Unit& unit) {
+#pragma unroll
+        for (int j = 0; j < 2; ++j)
+#pragma unroll
+            for (int g = 0; g < G; ++g)
+#pragma unroll
+                for (int i = 0; i < MT; ++i) acc[g][i] = __builtin_amdgcn_mfma_i32_16x16x64_i8(unit.w[g][j], unit.a[i][j], acc[g][i], 0, 0, 0);
+    };
+    // a ring of units: while one is multiplied the others are on their way
+    constexpr int RING = G * MT >= 16 ? 2 : G * MT >= 4 ? 3 : 4;
+    Unit ring[RING];
+#pragma unroll
+    for (int b = 0; b < RING; ++b)
+        if (b < count) load(ring[b], b);
+    int u = 0;
+    for (; u + 2 * RING <= count; u += RING)
+#pragma unroll
+        for (int b = 0; b < RING; ++b) {
+            multiply(ring[b]);
+            load(ring[b], u + b + RING);
+        }
+#pragma unroll
+    for (int b = 0; b < RING; ++b)
+        if (u + b < count) {
+            multiply(ring[b]);
+            if (u + b + RING < count) load(ring[b], u + b + RING);
+        }
+#pragma unroll
+    for (int b = 0; b < RING; ++b)
+        if (u + RING + b < count) multiply(ring[b]);
+
+    // the wavefronts' sums of a block, added by the wavefront that writes it
+#pragma unroll
+    for (int t0 = 0; t0 < G * MT; t0 += AT_ONCE) {
+        if (t0 > 0) __syncthreads();
+#pragma unroll
+        for (int t = 0; t < AT_ONCE; ++t) shared[wave][t][lane] = acc[(t0 + t) / MT][(t0 + t) % MT];
+        __syncthreads();
+        if (wave >= AT_ONCE) continue;
+        int4v sum = shared[0][wave][lane];
+#pragma unroll
+        for (int other = 1; other < WAVES; ++other) sum += shared[other][wave][lane];
+        const int group = first_group + (t0 + wave) / MT, block = (t0 + wave) % MT;
+        if (group >= groups || block * 16 >= M) continue;
+        if constexpr (PARTS) sums[(((long)part * ((M + 15) / 16) + block) * groups + group) * XRT_WAVE + lane] = sum;
+        else finish_block<MODE, TO>(sum, block * 16, group, to);
+    }
+}
+
+// ---- more rows --------------------------------------------------------------------------------------------------------------------------------------------
+
+constexpr int BN = 256;                // packed rows of w in a tile
+
+// Tiles of BM (256, 192 or 128) rows of a by 256 packed rows of w: eight wavefronts, two to a SIMD, which take turns as those of the bfloat16 product's large
+// tiles do. Of the two on a SIMD (one of each group of four) one reads the operands of its next products from LDS and asks for tiles to come while the other
+// multiplies; a barrier ends a turn, and the second group runs one barrier behind the first. A wavefront's part (BM / 2 x 64) is four quarters along k: (half
+// h of its rows of a, half g of its rows of w) in the order (0,0) (0,1) (1,1) (1,0), so that every turn reads one new half: w0, w1, a1, and a0 of the next
+// tile. A half is loaded into the place of the same half two tiles ago as soon as both groups have read that, seven quarters before it is needed, and the
+// waits leave the newer six quarters' loads in flight.
+//
+// height: the rows of a that a tile stands for, a multiple of 16 up to BM (even_height): the first four wavefronts take half of the blocks of 16, or one
+// more than the others, and a wavefront runs the loop made for its number of blocks (all, one or two fewer).
+template <int BM, int MODE, typename TO, bool PARTS>
+__global__ void __launch_bounds__(8 * XRT_WAVE) gemm_int8_large_kernel(const signed char* __restrict__ a, const signed char* __restrict__ w, int4v* __restrict__ sums,
+                                                                       int stride, int groups, int tiles_m, int tiles_n, int height, int by_parts,
+                                                                       int steps_a_part, const Result<TO> to) {
+    constexpr int STEP = XRT_INT8_STEP, WAVES_N = 4;
+    constexpr int WAVE_M = BM / 2, WAVE_N = BN / WAVES_N;      // the wavefront's part of the tile
+    constexpr int TM = WAVE_M / 16, TN = WAVE_N / 16, HM = TM / 2, HN = TN / 2;      // blocks of 16 rows of a and of w: all, and a half
+    constexpr int BLOCKS_A = BM / 16;                          // kilobytes of one half of a: where they do not divide among the wavefronts, the spare loads fetch the last one again
+    constexpr int LOADS_A = (BLOCKS_A + 7) / 8, LOADS_B = BN / 128;      // load instructions of a wavefront for one half
+    extern __shared__ __attribute__((aligned(16))) unsigned char lds_raw[];
+    unsigned char* stage_a = lds_raw;                          // [2][BM][128]: rows of eight 16-byte pieces, swizzled
+    unsigned char* stage_b = stage_a + 2 * BM * STEP;          // [2][16 groups][2][1024]: packed tiles as they lie
+    float* lds_a_scales = reinterpret_cast<float*>(stage_b + 2 * BN * STEP);      // [256] of the tile's rows
+    float* lds_w_scales = lds_a_scales + 256;                  // [256]
+
+    const PartPlace dealt = PARTS ? part_place(blockIdx.x, blockIdx.y, tiles_m, tiles_n, by_parts) : PartPlace{tile_place(blockIdx.x, tiles_m, tiles_n), 0};
+    if (dealt.tile.m < 0) return;
+    const int M = to.M, N = to.N;
+    const int m0 = dealt.tile.m * height, first_group = dealt.tile.n * (BN / 16);
+    const int lane = threadIdx.x % XRT_WAVE, wave = __builtin_amdgcn_readfirstlane(threadIdx.x / XRT_WAVE);
+    const int wave_m = wave / WAVES_N, wave_n = wave % WAVES_N;
+    const int quad = lane / 16;                                // which four packed rows of a block this lane has the sums of
+    const int upper_blocks = (height / 16 + 1) / 2;            // of 16 rows, of the wavefronts 0 to 3
+    const int blocks = wave_m == 0 ? upper_blocks : height / 16 - upper_blocks;
+    const int wave_row = m0 + wave_m * upper_blocks * 16, tile_end = min(m0 + height, M);
+    a += (long)m0 * stride;                                    // (offsets inside a tile fit 32 bits: 256 rows of up to 131072 bytes)
+    w += (long)first_group * 16 * stride;
+
+    // Piece c (16 bytes) of row r lies at place c ^ (r % 8) of the row: the lanes that a 16-byte read serves at once then take different banks.
+    // The kilobyte of LDS (8 rows of a, or a packed tile) that load i of half h fills, for a wavefront; rows: a wavefront's rows of the operand in the tile.
+    auto block_of = [&](int h, int i, int rows, int blocks) {
+        const int per = rows / 16, p = min(i * 8 + wave, blocks - 1);
+        return (p / per * rows + h * (rows / 2)) / 8 + p % per;
+    };
+    unsigned off_a[2][LOADS_A], off_b[2][LOADS_B];             // bytes
+    const int missing = WAVE_M - upper_blocks * 16;            // (rows of the tile that no wavefront has: the last one again, not multiplied)
+    const unsigned piece_of_lane = (unsigned)((lane % 8) ^ (lane / 8)) * 16u;
+#pragma unroll
+    for (int h = 0; h < 2; ++h)
+#pragma unroll
+        for (int i = 0; i < LOADS_A; ++i) {
+            const int block = block_of(h, i, WAVE_M, BLOCKS_A), row = block * 8 + lane / 8 - (block * 8 >= WAVE_M ? missing : 0);
+            off_a[h][i] = (unsigned)min(row, tile_end - 1 - m0) * (unsigned)stride + piece_of_lane;
+        }
+#pragma unroll
+    for (int h = 0; h < 2; ++h)
+#pragma unroll
+        for (int i = 0; i < LOADS_B; ++i) {
+            const int block = block_of(h, i, WAVE_N, BN / 16);
+            const int group = min(block / 2, groups - 1 - first_group);                    // groups beyond the matrix: the last one again
+            off_b[h][i] = (unsigned)group * 16u * (unsigned)stride + (unsigned)(block % 2) * 1024u + (unsigned)lane * 16u;
+        }
+    const unsigned lds_a0 = lds_address(stage_a), lds_b0 = lds_address(stage_b);
+    auto issue_a = [&](int h, int stage, int step) {
+#pragma unroll
+        for (int i = 0; i < LOADS_A; ++i)
+            load_to_lds(a, off_a[h][i] + (unsigned)step * 128u, lds_a0 + (unsigned)(stage * BM * STEP + block_of(h, i, WAVE_M, BLOCKS_A) * 1024));
+    };
+    auto issue_b = [&](int h, int stage, int step) {
+#pragma unroll
+        for (int i = 0; i < LOADS_B; ++i)
+            load_to_lds(w, off_b[h][i] + (unsigned)step * 2048u, lds_b0 + (unsigned)(stage * BN * STEP + block_of(h, i, WAVE_N, BN / 16) * 1024));
+    };
+    // the tile's scales, ahead of the tiles themselves: wavefronts 0 to 3 those of 64 rows of a each, 4 to 7 those of 64 packed rows of w
+    if constexpr (!PARTS) {
+        if (wave < 4) load_dword_to_lds(to.a_scales, (unsigned)min(m0 + wave * 64 + lane, M - 1) * 4u, lds_address(lds_a_scales + wave * 64));
+        else load_dword_to_lds(to.w_scales, (unsigned)min(first_group * 16 + (wave - 4) * 64 + lane, groups * 16 - 1) * 4u, lds_address(lds_w_scales + (wave - 4) * 64));
+    }
+    // where this lane finds its 16 bytes of block 0 of its wavefront, for either 64 columns of the tile
+    const unsigned char* place_a[2];
+    const unsigned char* place_b[2];
+#pragma unroll
+    for (int ks = 0; ks < 2; ++ks) {
+        place_a[ks] = stage_a + (wave_m * WAVE_M + lane % 16) * STEP + (((ks * 4 + quad) ^ (lane % 8)) * 16);
+        place_b[ks] = stage_b + wave_n * WAVE_N * STEP + ks * 1024 + lane * 16;
+    }
+    int4v xa[2][2][HM], wb[2][2][HN];                          // [half][64 columns][block]
+    // (T: the blocks of the wavefront, TM or somewhat fewer; they are missing from the second half)
+    auto read_a = [&](auto t, int h, int stage) {
+        constexpr int T = decltype(t)::value;
+#pragma unroll
+        for (int ks = 0; ks < 2; ++ks)
+#pragma unroll
+            for (int i = 0; i < HM; ++i)
+                if (h * HM + i < T) xa[h][ks][i] = *reinterpret_cast<const int4v*>(place_a[ks] + stage * BM * STEP + (h * HM + i) * 16 * STEP);
+    };
+    auto read_b = [&](int h, int stage) {
+#pragma unroll
+        for (int ks = 0; ks < 2; ++ks)
+#pragma unroll
+            for (int j = 0; j < HN; ++j)
+                wb[h][ks][j] = *reinterpret_cast<const int4v*>(place_b[ks] + stage * BN * STEP + (h * HN + j) * 16 * STEP);
+    };
+    int4v acc[TM][TN];
+#pragma unroll
+    for (int i = 0; i < TM; ++i)
+#pragma unroll
+        for (int j = 0; j < TN; ++j) acc[i][j] = int4v{0, 0, 0, 0};
+    auto multiply = [&](auto t, int h, int g) {
+        constexpr int T = decltype(t)::value;
+#pragma unroll
+        for (int ks = 0; ks < 2; ++ks)
+#pragma unroll
+            for (int i = 0; i < HM; ++i)
+#pragma unroll
+                for (int j = 0; j < HN; ++j)
+                    if (h * HM + i < T)
+                        acc[h * HM + i][g * HN + j] = __builtin_amdgcn_mfma_i32_16x16x64_i8(wb[g][ks][j], xa[h][ks][i], acc[h * HM + i][g * HN + j], 0, 0, 0);
+    };
+    const int first_step = dealt.part * steps_a_part;
+    const int steps = min(steps_a_part, stride / STEP - first_step), last_step = first_step + steps - 1;
+    auto step_of = [&](int t) { return min(first_step + t, last_step); };        // (tiles beyond the end: the last one again, into a place nobody reads)
+#pragma unroll
+    for (int t = 0; t < 2; ++t) {
+        issue_a(0, t, step_of(t));
+        issue_b(0, t, step_of(t));
+        issue_b(1, t, step_of(t));
+        issue_a(1, t, step_of(t));
+    }
+    // Loads that may stay in flight behind a quarter's reads: those of the six quarters after the next one.
+    constexpr int ALL = 2 * (LOADS_A + LOADS_B);
+    auto barrier = [] {
+        __builtin_amdgcn_sched_barrier(0);
+        asm volatile("s_barrier" ::: "memory");
+        __builtin_amdgcn_sched_barrier(0);
+    };
+    auto walk = [&](auto t_blocks) {
+        wait_loads_and_barrier<ALL + LOADS_A + LOADS_B>();     // a0 and w0 of tile 0 are in LDS
+        read_a(t_blocks, 0, 0);
+        wait_loads_and_barrier<ALL + LOADS_A + LOADS_B>();     // and a0 is read by all: the first turn fills its place again
+        auto turn = [&](auto in_flight, int h, int g) {
+            __builtin_amdgcn_sched_barrier(0);
+            wait_loads_and_barrier<decltype(in_flight)::value>();  // this wavefront's reads are done: what it read may be overwritten
+            __builtin_amdgcn_sched_barrier(0);
+            multiply(t_blocks, h, g);
+            barrier();
+        };
+        if (wave >= 4) barrier();
+        for (int t = 0; t < steps; ++t) {
+            const int now = t % 2, next = step_of(t + 2);
+            read_b(0, now);
+            issue_a(0, now, next);
+            turn(std::integral_constant<int, ALL + 2 * LOADS_A>{}, 0, 0);           // in flight: a1 a0 w0 w1 a1 a0
+            read_b(1, now);
+            issue_b(0, now, next);
+            turn(std::integral_constant<int, ALL + LOADS_A + LOADS_B>{}, 0, 1);     // a0 w0 w1 a1 a0 w0
+            read_a(t_blocks, 1, now);
+            issue_b(1, now, next);
+            turn(std::integral_constant<int, ALL + 2 * LOADS_B>{}, 1, 1);           // w0 w1 a1 a0 w0 w1
+            read_a(t_blocks, 0, now ^ 1);
+            issue_a(1, now, next);
+            turn(std::integral_constant<int, ALL + LOADS_A + LOADS_B>{}, 1, 0);     // w1 a1 a0 w0 w1 a1
+        }
+    };
+    if (BM == 128 || blocks == TM) walk(std::integral_constant<int, TM>{});
+    else if (blocks == TM - 1) walk(std::integral_constant<int, TM - 1>{});
+    else walk(std::integral_constant<int, TM - 2>{});          // (fewer than that: some products that nobody writes)
+    if (wave < 4) barrier();
+    wait_loads_and_barrier<0>();                               // nothing lands in LDS after this
+
+    // ---- epilogue: element e of acc[i][j] is row i * 16 + lane % 16 of a and packed row j * 16 + quad * 4 + e of w
+    const int row_end = min(wave_row + blocks * 16, tile_end);           // of the wavefront's rows
+    const int wave_group = first_group + wave_n * TN;
+    if constexpr (PARTS) {
+#pragma unroll
+        for (int i = 0; i < TM; ++i)
+#pragma unroll
+            for (int j = 0; j < TN; ++j)
+                if (wave_row + i * 16 < row_end && wave_group + j < groups)
+                    sums[(((long)dealt.part * ((M + 15) / 16) + wave_row / 16 + i) * groups + wave_group + j) * XRT_WAVE + lane] = acc[i][j];
+        return;
+    }
+    float4 w_scale[TN];
+    float a_scale[TM];
+#pragma unroll
+    for (int j = 0; j < TN; ++j) w_scale[j] = *reinterpret_cast<const float4*>(lds_w_scales + wave_n * WAVE_N + j * 16 + quad * 4);
+#pragma unroll
+    for (int i = 0; i < TM; ++i) a_scale[i] = lds_a_scales[min(wave_row - m0 + i * 16 + lane % 16, 255)];
+    auto value = [&](int i, int j, int e) {
+        const float of_channel = e == 0 ? w_scale[j].x : e == 1 ? w_scale[j].y : e == 2 ? w_scale[j].z : w_scale[j].w;
+        return scaled(acc[i][j][e], a_scale[i], of_channel);
+    };
+    TO* out = to.out;
+    if constexpr (MODE == MODE_GATED) {
+        // A group of 16 packed rows holds the gate rows of 8 outputs, then their up rows: the lane with an output's up sum
+        // is 32 lanes away. One exchange of half a register between the sums of two blocks of a leaves gate and up of
+        // every output of both in one lane (lanes 0 to 31 the first block's outputs, the others the second's); for
+        // bfloat16 another one between two groups of w brings eight neighbouring outputs together: 16 bytes a store.
+        const long n_wave = (long)wave_group * 8;
+        const bool wide = N % 8 == 0 && (uintptr_t)out % 16 == 0;
+#pragma unroll
+        for (int i = 0; i < TM; i += 2) {
+            const long m = wave_row + lane % 16 + i * 16 + lane / 32 * 16;
+#pragma unroll
+            for (int j = 0; j < TN; j += 2) {
+                float made[2][4];
+#pragma unroll
+                for (int u = 0; u < 2; ++u)
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) {
+                        float gate = value(i, j + u, e), up = value(i + 1, j + u, e);
+                        exchange_halves(gate, up);
+                        made[u][e] = gate_activation<sizeof(TO) == 2>(gate, to.activation) * up;
+                    }
+                if constexpr (sizeof(TO) == 2) {
+                    if (wide) {
+                        const uint4v piece = join_rows<TO>(made[0], made[1]);
+                        const long n = n_wave + (j + quad % 2) * 8;
+                        if (m < row_end && n < N) *reinterpret_cast<uint4v*>(out + m * (long)N + n) = piece;
+                        continue;
+                    }
+                }
+#pragma unroll
+                for (int u = 0; u < 2; ++u) store_four<TO>(out, m, n_wave + (j + u) * 8 + quad % 2 * 4, row_end, N, made[u], wide);
             }
-            if (mine && n < N) {
-                TO* to = out + m * N + n;
-                if constexpr (MODE == MODE_ACCUMULATE) value += to_float(*to);
-                *to = from_float<TO>(value);
+        }
+    } else {
+        const bool wide = N % 8 == 0 && (uintptr_t)out % 16 == 0;
+        // Two neighbouring blocks of columns change eight lanes with each other, so that an instruction takes eight rows of
+        // 128 bytes, whole cache lines, instead of sixteen of 64.
+        const long row8 = wave_row + lane % 8;
+        const int upper = lane % 16 / 8;
+        if constexpr (MODE == MODE_STORE && sizeof(TO) == 2) {
+            if (wide) {
+                static_assert(TN == 4, "two pieces of 32 columns");
+                const long n = (long)wave_group * 16 + (2 * upper + quad % 2) * 16 + quad / 2 * 8;
+#pragma unroll
+                for (int i = 0; i < TM; ++i) {
+                    uint4v piece[2];
+#pragma unroll
+                    for (int u = 0; u < 2; ++u) {
+                        const float first[4] = {value(i, 2 * u, 0), value(i, 2 * u, 1), value(i, 2 * u, 2), value(i, 2 * u, 3)};
+                        const float second[4] = {value(i, 2 * u + 1, 0), value(i, 2 * u + 1, 1), value(i, 2 * u + 1, 2), value(i, 2 * u + 1, 3)};
+                        piece[u] = join_rows<TO>(first, second);
+                    }
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) {
+                        unsigned low = piece[0][e], high = piece[1][e];
+                        exchange_eights(low, high);
+                        piece[0][e] = low;
+                        piece[1][e] = high;
+                    }
+#pragma unroll
+                    for (int u = 0; u < 2; ++u) {
+                        const long m = row8 + i * 16 + u * 8;
+                        if (m < row_end && n < N) *reinterpret_cast<uint4v*>(out + m * (long)N + n) = piece[u];
+                    }
+                }
+                return;
             }
+        }
+        constexpr int RUN = TM % 4 == 0 ? 4 : 3;               // blocks of a whose old values are read in one go, before any is written
+#pragma unroll
+        for (int i0 = 0; i0 < TM; i0 += RUN) {
+            float before[RUN][TN][4];
+            if constexpr (MODE == MODE_ACCUMULATE) {
+#pragma unroll
+                for (int i = 0; i < RUN; ++i)
+#pragma unroll
+                    for (int j = 0; j < TN; ++j)
+                        load_four<TO>(out, row8 + (i0 + i) * 16 + j % 2 * 8, (long)(wave_group + j / 2 * 2 + upper) * 16 + quad * 4, row_end, N, before[i][j], wide);
+            }
+#pragma unroll
+            for (int i = 0; i < RUN; ++i)
+#pragma unroll
+                for (int j = 0; j < TN; j += 2) {
+                    float made[2][4];
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) {
+                        made[0][e] = value(i0 + i, j, e);
+                        made[1][e] = value(i0 + i, j + 1, e);
+                        exchange_eights(made[0][e], made[1][e]);
+                        if constexpr (MODE == MODE_ACCUMULATE) {
+                            made[0][e] = before[i][j][e] + made[0][e];
+                            made[1][e] = before[i][j + 1][e] + made[1][e];
+                        }
+                    }
+                    const long n = (long)(wave_group + j + upper) * 16 + quad * 4;
+                    store_four<TO>(out, row8 + (i0 + i) * 16, n, row_end, N, made[0], wide);
+                    store_four<TO>(out, row8 + (i0 + i) * 16 + 8, n, row_end, N, made[1], wide);
+                }
         }
     }
 }
 
+// ---- which kernel -----------------------------------------------------------------------------------------------------------------------------------------
+
+struct Plan {
+    int tile;           // rows of a of a tile (256, 192, 128), or 0: the kernel of few rows
+    int blocks;         // of 16 rows of a, of the kernel of few rows (1, 2 or 4)
+    int groups;         // of w a workgroup, of the same (1, 2 or 4)
+    int parts;          // of k
+};
+
+Plan plan_of(long M, long groups, long stride) {
+    const long units = stride / XRT_INT8_STEP;
+    if (M <= 64) {
+        Plan plan{0, M <= 16 ? 1 : M <= 32 ? 2 : 4, 1, 1};
+        plan.groups = groups >= 1024 ? plan.blocks : 1;
+        const long workgroups = (groups + plan.groups - 1) / plan.groups;
+        while (plan.parts < 8 && workgroups * plan.parts * 2 <= XRT_COMPUTE_UNITS && units / (plan.parts * 2) >= 8) plan.parts *= 2;
+        return plan;
+    }
+    Plan plan{0, 0, 0, 1};
+    const long tiles_n = (groups + 15) / 16;
+    double best = 0;
+    for (const int tile : {256, 192, 128}) {
+        const long tiles = (M + tile - 1) / tile * tiles_n;
+        const long rounds = (tiles + XRT_COMPUTE_UNITS - 1) / XRT_COMPUTE_UNITS;
+        const double cost = rounds * (even_height((int)M, tile) + 32.0);
+        if (plan.tile == 0 || cost < best) plan.tile = tile, best = cost;
+    }
+    const long tiles = (M + plan.tile - 1) / plan.tile * tiles_n;
+    while (plan.parts < 16 && tiles * plan.parts * 2 <= XRT_COMPUTE_UNITS && units / (plan.parts * 2) >= 4) plan.parts *= 2;
+    return plan;
+}
+
+long sums_bytes(const Plan& plan, long M, long groups) { return plan.parts == 1 ? 0 : plan.parts * ((M + 15) / 16) * groups * XRT_WAVE * (long)sizeof(int4v); }
+
+struct Operands { const signed char* a; const signed char* w; int4v* sums; int stride, groups; hipStream_t stream; };
+
+template <int MT, int G, int MODE, typename TO>
+void launch_few(const Operands& o, const Plan& plan, const Result<TO>& to) {
+    const dim3 grid((o.groups + G - 1) / G, plan.parts);
+    if (plan.parts == 1) gemm_int8_few_kernel<MT, G, MODE, TO, false><<<grid, WAVES * XRT_WAVE, 0, o.stream>>>(o.a, o.w, nullptr, to.M, o.stride, o.groups, 1, to);
+    else gemm_int8_few_kernel<MT, G, MODE_STORE, float, true><<<grid, WAVES * XRT_WAVE, 0, o.stream>>>(o.a, o.w, o.sums, to.M, o.stride, o.groups, plan.parts, Result<float>{});
+}
+
+template <int BM, int MODE, typename TO, bool PARTS>
+int launch_large(const Operands& o, const Plan& plan, const Result<TO>& to) {
+    constexpr size_t lds = (size_t)2 * (BM + BN) * XRT_INT8_STEP + 2 * 256 * sizeof(float);
+    auto kernel = gemm_int8_large_kernel<BM, MODE, TO, PARTS>;
+    static bool configured[64] = {};                           // per instantiation and device
+    int device = 0;
+    XRT_REQUIRE(hipGetDevice(&device) == hipSuccess, "linear_int8: no current device");
+    if (device < 0 || device >= 64 || !configured[device]) {
+        const hipError_t e = hipFuncSetAttribute(reinterpret_cast<const void*>(kernel), hipFuncAttributeMaxDynamicSharedMemorySize, (int)lds);
+        XRT_REQUIRE(e == hipSuccess, "linear_int8: cannot reserve %zu bytes of LDS: %s", lds, hipGetErrorString(e));
+        if (device >= 0 && device < 64) configured[device] = true;
+    }
+    const int units = o.stride / XRT_INT8_STEP, steps = (units + plan.parts - 1) / plan.parts;
+    const int height = even_height(to.M, BM), tiles_m = (to.M + height - 1) / height, tiles_n = (o.groups + 15) / 16;
+    const long ids = part_ids((long)tiles_m * tiles_n, plan.parts, true);        // a whole number of rounds over the XCDs
+    XRT_REQUIRE(ids < (1L << 31), "linear_int8: %ld tiles", ids);
+    kernel<<<(unsigned)ids, 8 * XRT_WAVE, lds, o.stream>>>(o.a, o.w, o.sums, o.stride, o.groups, tiles_m, tiles_n, height, plan.parts, steps, to);
+    return 0;
+}
+
+template <int MODE, typename TO>
+int launch(const Operands& o, const Plan& plan, const Result<TO>& to) {
+    int failed = 0;
+    if (plan.tile == 0) {
+        const int kind = plan.blocks * 8 + plan.groups;
+        if (kind == 8 + 1) launch_few<1, 1, MODE, TO>(o, plan, to);
+        else if (kind == 16 + 1) launch_few<2, 1, MODE, TO>(o, plan, to);
+        else if (kind == 16 + 2) launch_few<2, 2, MODE, TO>(o, plan, to);
+        else if (kind == 32 + 1) launch_few<4, 1, MODE, TO>(o, plan, to);
+        else launch_few<4, 4, MODE, TO>(o, plan, to);
+    } else if (plan.parts > 1) {
+        Result<float> sizes{};
+        sizes.M = to.M, sizes.N = to.N;
+        if (plan.tile == 256) failed = launch_large<256, MODE_STORE, float, true>(o, plan, sizes);
+        else if (plan.tile == 192) failed = launch_large<192, MODE_STORE, float, true>(o, plan, sizes);
+        else failed = launch_large<128, MODE_STORE, float, true>(o, plan, sizes);
+    } else if (plan.tile == 256) failed = launch_large<256, MODE, TO, false>(o, plan, to);
+    else if (plan.tile == 192) failed = launch_large<192, MODE, TO, false>(o, plan, to);
+    else failed = launch_large<128, MODE, TO, false>(o, plan, to);
+    if (failed) return failed;
+    if (plan.parts > 1) {
+        const long blocks = (long)((to.M + 15) / 16) * o.groups;
+        int8_finish_kernel<MODE, TO><<<(unsigned)((blocks + 3) / 4), 256, 0, o.stream>>>(o.sums, plan.parts, o.groups, blocks, to);
+    }
+    XRT_LAUNCH_CHECK("linear_int8");
+    return 0;
+}
+
 }  // namespace
 
-extern "C" long xrt_linear_int8_workspace(int M, int N, int K, int mode) { return 0; }
+extern "C" long xrt_linear_int8_workspace(int M, int N, int K, int mode) {
+    if (M <= 0 || N <= 0 || K <= 0 || K > XRT_INT8_MOST_K) return 0;
+    const long groups = int8_groups(N, mode_of(mode) == MODE_GATED);
+    return sums_bytes(plan_of(M, groups, int8_stride(K)), M, groups);
+}
 
 extern "C" int xrt_linear_int8(const void* a, const float* a_scales, const void* w, const float* w_scales, void* out, int out_dtype, int M, int N, int K,
                                int mode, void* workspace, long workspace_bytes, void* stream) {
     XRT_REQUIRE(M >= 0 && N > 0 && K > 0 && K <= XRT_INT8_MOST_K && (M == 0 || (a && a_scales && w && w_scales && out)), "linear_int8: bad operands M=%d N=%d K=%d", M, N, K);
-    XRT_REQUIRE(mode_of(mode) >= MODE_STORE && mode_of(mode) <= MODE_GATED && activation_of(mode) < XRT_ACT_COUNT && (mode_of(mode) == MODE_GATED || activation_of(mode) == 0),
+    const int kind = mode_of(mode);
+    XRT_REQUIRE(kind >= MODE_STORE && kind <= MODE_GATED && activation_of(mode) >= 0 && activation_of(mode) < XRT_ACT_COUNT && (kind == MODE_GATED || activation_of(mode) == 0),
                 "linear_int8: unknown mode %d", mode);
-    XRT_REQUIRE(out_dtype == XRT_F32 || (out_dtype == XRT_BF16 && mode_of(mode) != MODE_ACCUMULATE), "linear_int8: unknown element type %d of out for mode %d", out_dtype, mode);
+    XRT_REQUIRE(out_dtype == XRT_F32 || (out_dtype == XRT_BF16 && kind != MODE_ACCUMULATE), "linear_int8: unknown element type %d of out for mode %d", out_dtype, mode);
+    XRT_REQUIRE(((uintptr_t)a | (uintptr_t)w | (uintptr_t)w_scales) % 16 == 0, "linear_int8: rows, weights and their scales start at multiples of 16 bytes");
     if (M == 0) return 0;
-    const bool gated = mode_of(mode) == MODE_GATED;
-    const int stride = (int)int8_stride(K), groups = (int)int8_groups(N, gated);
-    XRT_REQUIRE((M + 63) / 64 <= XRT_GRID_ROWS, "linear_int8: too many rows, %d", M);
-    const dim3 grid((groups + 3) / 4, (M + 63) / 64);
-    hipStream_t s = (hipStream_t)stream;
-#define XRT_INT8(MODE, TO) gemm_int8_kernel<MODE, TO><<<grid, 256, 0, s>>>((const signed char*)a, a_scales, (const signed char*)w, w_scales, (TO*)out, M, N, stride, groups, activation_of(mode))
-    if (gated && out_dtype == XRT_F32) XRT_INT8(MODE_GATED, float);
-    else if (gated) XRT_INT8(MODE_GATED, bf16);
-    else if (mode_of(mode) == MODE_ACCUMULATE) XRT_INT8(MODE_ACCUMULATE, float);
-    else if (out_dtype == XRT_F32) XRT_INT8(MODE_STORE, float);
-    else XRT_INT8(MODE_STORE, bf16);
-#undef XRT_INT8
-    XRT_LAUNCH_CHECK("linear_int8");
-    return 0;
+    const long groups = int8_groups(N, kind == MODE_GATED);
+    const Plan plan = plan_of(M, groups, int8_stride(K));
+    const long need = sums_bytes(plan, M, groups);
+    XRT_REQUIRE(need == 0 || (workspace && workspace_bytes >= need && (uintptr_t)workspace % 16 == 0), "linear_int8: a workspace of %ld bytes is needed, %ld given", need, workspace ? workspace_bytes : 0);
+    XRT_REQUIRE((long)M + 256 < (1L << 31) && groups * 16 < (1L << 30), "linear_int8: too many rows, %d of a and %d of w", M, N);
+    const Operands o{(const signed char*)a, (const signed char*)w, (int4v*)workspace, (int)int8_stride(K), (int)groups, (hipStream_t)stream};
+    if (out_dtype == XRT_BF16) {
+        const Result<bf16> to{a_scales, w_scales, (bf16*)out, M, N, activation_of(mode)};
+        return kind == MODE_GATED ? launch<MODE_GATED, bf16>(o, plan, to) : launch<MODE_STORE, bf16>(o, plan, to);
+    }
+    const Result<float> to{a_scales, w_scales, (float*)out, M, N, activation_of(mode)};
+    return kind == MODE_GATED ? launch<MODE_GATED, float>(o, plan, to) : kind == MODE_ACCUMULATE ? launch<MODE_ACCUMULATE, float>(o, plan, to) : launch<MODE_STORE, float>(o, plan, to);
 }
