@@ -398,8 +398,9 @@ def test_refusals(ops):
         lambda: ops.linear_int8(x, w, rand(4, 20)), lambda: ops.linear_int8(q, rand(20, 100), rand(4, 20)), lambda: ops.linear_int8(q, gated, rand(4, 20)),
         lambda: ops.linear_int8(q, w, rand(4, 21)), lambda: ops.linear_int8(q, w, rand(3, 20)), lambda: ops.linear_int8(ops.int8_rows(4, 99, DEV), w, rand(4, 20)),
         lambda: ops.linear_int8(q, w, rand(4, 20).bfloat16(), accumulate=True), lambda: ops.linear_int8(q, w, rand(4, 20).half()),
-        lambda: ops.linear_int8(q, w, rand(4, 40)[:, ::2]), lambda: ops.linear_int8(Int8Rows(q.values[:, :100], q.scales, 100), w, rand(4, 20)),
-        lambda: ops.linear_int8(Int8Rows(q.values, q.scales[:3], 100), w, rand(4, 20)), lambda: ops.linear_int8(Int8Rows(q.values, q.scales.cpu(), 100), w, rand(4, 20)),
+        lambda: ops.linear_int8(q, w, rand(4, 40)[:, ::2]), lambda: Int8Rows(q.values[:, :100], q.scales, 100), lambda: Int8Rows(q.values.cpu(), q.scales, 100), lambda: Int8Rows(q.values[0], q.scales, 100), lambda: Int8Rows(q.values, q.scales, 129),
+        lambda: Int8Rows(q.values.view(-1)[:-1].clone(), q.scales, 100), lambda: Int8Rows(torch.empty(4 * 128 + 8, dtype=torch.int8, device=DEV)[8:].view(4, 128), q.scales, 100),
+        lambda: Int8Rows(q.values, q.scales[:3], 100), lambda: Int8Rows(q.values, q.scales.cpu(), 100), lambda: Int8Rows(q.values, q.scales, 0),
         lambda: ops.linear_glu_int8(q, w, rand(4, 10)), lambda: ops.linear_glu_int8(q, gated, rand(4, 20)), lambda: ops.linear_glu_int8(q, gated, rand(4, 10), activation="relu"),
     ]
     for index, call in enumerate(refused):

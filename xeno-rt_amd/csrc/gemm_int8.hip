@@ -480,10 +480,10 @@ struct Plan {
 Plan plan_of(long M, long groups, long stride) {
     const long units = stride / XRT_INT8_STEP;
     if (M <= 64) {
-        Plan plan{0, M <= 16 ? 1 : M <= 32 ? 2 : 4, 1, 1};
-        plan.groups = groups >= 1024 ? plan.blocks : 1;
+        const int blocks = M <= 16 ? 1 : M <= 32 ? 2 : 4;
+        Plan plan{0, blocks, blocks, 1};
         const long workgroups = (groups + plan.groups - 1) / plan.groups;
-        while (plan.parts < 8 && workgroups * plan.parts * 2 <= XRT_COMPUTE_UNITS && units / (plan.parts * 2) >= 8) plan.parts *= 2;
+        while (plan.parts < 8 && workgroups * plan.parts * 2 <= (blocks == 1 ? XRT_COMPUTE_UNITS / 2 : XRT_COMPUTE_UNITS) && units / (plan.parts * 2) >= 8) plan.parts *= 2;
         return plan;
     }
     Plan plan{0, 0, 0, 1};

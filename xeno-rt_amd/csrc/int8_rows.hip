@@ -24,6 +24,19 @@ __device__ __forceinline__ void load_eight(const T* row, int at, int width, floa
         for (int e = 0; e < 8; ++e) v[e] = at + e < width ? to_float(row[at + e]) : 0.f;
     }
 }
+template <typename T>
+__device__ __forceinline__ void store_eight(T* row, int at, int width, const float (&v)[8]) {
+    Eight<T> piece;
+#pragma unroll
+    for (int e = 0; e < 8; ++e) piece.e[e] = from_float<T>(v[e]);
+    if (at + 8 <= width) {
+        __builtin_memcpy(row + at, &piece, sizeof(piece));
+    } else {
+#pragma unroll
+        for (int e = 0; e < 8; ++e)
+            if (at + e < width) row[at + e] = piece.e[e];
+    }
+}
 
 // The bits of |v|: as whole numbers they are ordered as the magnitudes are, infinity above all numbers and NaN above infinity.
 __device__ __forceinline__ unsigned magnitude_bits(float v) { return __builtin_bit_cast(unsigned, v) & 0x7fffffffu; }
@@ -48,25 +61,34 @@ __device__ __forceinline__ float scale_of(unsigned most) {
     return most >= 0x7f800000u ? __builtin_nanf("") : __builtin_bit_cast(float, most) / 127.0f;
 }
 
-// Eight values as signed bytes. (A scale too small for a normal float32 is off by up to half of itself: the quotients are clamped.)
+// Eight values as signed bytes. The quotient by the scale's reciprocal, corrected by what is left of the value (exact, by a fused multiply-add), is the
+// division's own result where neither leaves the normal numbers: four instructions instead of twelve. Adding 1.5 * 2^23 rounds it to an integer, halves to
+// even, whose two's complement then stands in the sum's lowest bits.
 __device__ __forceinline__ uint2 eight_bytes(const float (&y)[8], float scale) {
     unsigned word[2] = {0u, 0u};
-    if (scale > 0.f) {                                          // (neither zero nor NaN)
+    if (scale >= 0x1p-100f && scale <= 0x1p100f) {
+        const float inverse = 1.0f / scale;
+        unsigned bits[8];
 #pragma unroll
         for (int e = 0; e < 8; ++e) {
-            const float q = fminf(fmaxf(rintf(y[e] / scale), -127.f), 127.f);
-            word[e / 4] |= ((unsigned)(int)q & 255u) << (e % 4 * 8);
+            const float near = y[e] * inverse;
+            bits[e] = __builtin_bit_cast(unsigned, fmaf(fmaf(-near, scale, y[e]), inverse, near) + 0x1.8p23f);
         }
+#pragma unroll
+        for (int h = 0; h < 2; ++h)                             // the lowest bytes of four words, side by side
+            word[h] = __builtin_amdgcn_perm(bits[4 * h + 1], bits[4 * h], 0x0c0c0400u) | __builtin_amdgcn_perm(bits[4 * h + 3], bits[4 * h + 2], 0x04000c0cu);
+    } else if (scale > 0.f) {                                   // (neither zero nor NaN; a scale that is no normal number is off by up to half of itself)
+#pragma unroll
+        for (int e = 0; e < 8; ++e) word[e / 4] |= ((unsigned)(int)fminf(fmaxf(rintf(y[e] / scale), -127.f), 127.f) & 255u) << (e % 4 * 8);
     }
     return make_uint2(word[0], word[1]);
 }
 
-constexpr int PIECES = 4;            // pieces of eight elements that a thread keeps in registers
 constexpr int MOST_THREADS = 1024;
 
-// One workgroup a row. NORM: the row of x gets delta added (written back) and is normed before it is brought to 8 bits. A row wider than what the
+// One workgroup a row; PIECES: pieces of eight elements that a thread keeps in registers. NORM: the row of x gets delta added (written back) and is normed before it is brought to 8 bits. A row wider than what the
 // threads keep is read again for what comes after the sums.
-template <typename TX, typename TD, typename TW, bool NORM>
+template <typename TX, typename TD, typename TW, bool NORM, int PIECES>
 __global__ void __launch_bounds__(MOST_THREADS) int8_rows_kernel(TX* x, const TD* delta, const TW* __restrict__ weight, const int* __restrict__ rows,
                                                                  signed char* __restrict__ values, float* __restrict__ scales, long x_stride,
                                                                  int x_rows, int width, int stride, float eps) {
@@ -83,10 +105,14 @@ __global__ void __launch_bounds__(MOST_THREADS) int8_rows_kernel(TX* x, const TD
     TX* row = x + source * x_stride;
     const TD* add = NORM && delta ? delta + source * width : nullptr;
     const int step = blockDim.x * 8, first = threadIdx.x * 8;
-    float kept[PIECES][8];
+    constexpr bool EARLY = NORM && PIECES <= 2;                 // the gains are asked for now, so that they arrive under the sum
+    float kept[PIECES][8], gains[EARLY ? PIECES : 1][8];
     float inv_rms = 1.f;
 #pragma unroll
     for (int i = 0; i < PIECES; ++i) load_eight(row, first + i * step, width, kept[i]);
+    if constexpr (EARLY)
+#pragma unroll
+        for (int i = 0; i < PIECES; ++i) load_eight(weight, first + i * step, width, gains[i]);
     if constexpr (NORM) {
         auto added = [&](int at, float (&v)[8]) {
             if (!add || at >= width) return;
@@ -94,14 +120,7 @@ __global__ void __launch_bounds__(MOST_THREADS) int8_rows_kernel(TX* x, const TD
             load_eight(add, at, width, d);
 #pragma unroll
             for (int e = 0; e < 8; ++e) v[e] += d[e];
-            if (at + 8 <= width) {
-                Eight<TX> piece;
-#pragma unroll
-                for (int e = 0; e < 8; ++e) piece.e[e] = from_float<TX>(v[e]);
-                __builtin_memcpy(row + at, &piece, sizeof(piece));
-            } else {
-                for (int e = 0; at + e < width; ++e) row[at + e] = from_float<TX>(v[e]);
-            }
+            store_eight(row, at, width, v);
         };
         float sum = 0.f;
 #pragma unroll
@@ -120,18 +139,22 @@ __global__ void __launch_bounds__(MOST_THREADS) int8_rows_kernel(TX* x, const TD
         inv_rms = 1.0f / sqrtf(block_sum(sum, sums) / (float)width + eps);
     }
     // what is brought to 8 bits, of what the row holds (a thread reads again only what it wrote itself)
+    auto times = [&](float (&v)[8], const float (&gain)[8]) {
+#pragma unroll
+        for (int e = 0; e < 8; ++e) v[e] = v[e] * inv_rms * gain[e];
+    };
     auto finished = [&](int at, float (&v)[8]) {
         if constexpr (NORM) {
             float gain[8];
             load_eight(weight, at, width, gain);
-#pragma unroll
-            for (int e = 0; e < 8; ++e) v[e] = v[e] * inv_rms * gain[e];
+            times(v, gain);
         }
     };
     unsigned most = 0u;
 #pragma unroll
     for (int i = 0; i < PIECES; ++i) {
-        finished(first + i * step, kept[i]);
+        if constexpr (EARLY) times(kept[i], gains[i]);
+        else finished(first + i * step, kept[i]);
 #pragma unroll
         for (int e = 0; e < 8; ++e) most = max(most, magnitude_bits(kept[i][e]));
     }
@@ -155,23 +178,19 @@ __global__ void __launch_bounds__(MOST_THREADS) int8_rows_kernel(TX* x, const TD
     if (threadIdx.x == 0) scales[r] = scale;
 }
 
-// out[m][j] = values[m][j] * scales[m]: a thread eight neighbouring columns
+// out[m][j] = values[m][j] * scales[m]: `lanes` threads a row (a power of two up to 256), a thread eight neighbouring columns
 template <typename TO>
 __global__ void __launch_bounds__(256) int8_values_kernel(const signed char* __restrict__ values, const float* __restrict__ scales, TO* __restrict__ out,
-                                                          int rows, int width, int stride) {
-    const long pieces = (width + 7) / 8, id = (long)blockIdx.x * blockDim.x + threadIdx.x;
-    const long r = id / pieces;
-    if (r >= rows) return;
-    const int at = (int)(id % pieces) * 8;
-    const uint2 bytes = *reinterpret_cast<const uint2*>(values + r * stride + at);
+                                                          int rows, int width, int stride, int lanes) {
+    const long r = (long)blockIdx.x * (256 / lanes) + threadIdx.x / lanes;
+    const int at = ((int)blockIdx.y * lanes + (int)threadIdx.x % lanes) * 8;
+    if (r >= rows || at >= width) return;
     const float scale = scales[r];
-    TO* row = out + r * width;
-    Eight<TO> piece;
+    const uint2 bytes = *reinterpret_cast<const uint2*>(values + r * stride + at);
+    float v[8];
 #pragma unroll
-    for (int e = 0; e < 8; ++e) piece.e[e] = from_float<TO>((float)(int)(signed char)((e < 4 ? bytes.x : bytes.y) >> (e % 4 * 8)) * scale);
-    if (at + 8 <= width) __builtin_memcpy(row + at, &piece, sizeof(piece));
-    else
-        for (int e = 0; at + e < width; ++e) row[at + e] = piece.e[e];
+    for (int e = 0; e < 8; ++e) v[e] = (float)(int)(signed char)((e < 4 ? bytes.x : bytes.y) >> (e % 4 * 8)) * scale;
+    store_eight(out + r * width, at, width, v);
 }
 
 // A thread a 16-byte piece of the packed matrix; the threads of the first tile of a group see to its scales.
@@ -193,12 +212,8 @@ __global__ void __launch_bounds__(256) int8_pack_kernel(const signed char* __res
     if (tile % tiles == 0 && lane < 16) packed_scales[group * 16 + within] = there ? scales[row] : 0.f;
 }
 
-// Threads of a row's workgroup: two pieces of eight a thread, or what keeps the row in registers, if it can be.
-int threads_for(int stride) {
-    const int pieces = stride / 8;
-    const int wanted = pieces <= 2 * MOST_THREADS ? (pieces + 1) / 2 : MOST_THREADS;
-    return whole_wavefronts(wanted);
-}
+// Threads of a row's workgroup, where each keeps up to `most` pieces.
+int threads_for(int stride, int most) { return whole_wavefronts(min(MOST_THREADS, (stride / 8 + most - 1) / most)); }
 
 }  // namespace
 
@@ -210,12 +225,16 @@ extern "C" int xrt_quantize_int8(const void* x, int dtype, long x_stride, void* 
     XRT_REQUIRE(dtype == XRT_F32 || dtype == XRT_BF16, "quantize_int8: unknown dtype %d", dtype);
     XRT_REQUIRE(x_stride >= k, "quantize_int8: rows of %d elements %ld apart", k, x_stride);
     if (rows == 0) return 0;
-    const int stride = (int)int8_stride(k), threads = threads_for(stride);
+    const int stride = (int)int8_stride(k);
     hipStream_t s = (hipStream_t)stream;
-    if (dtype == XRT_F32)
-        int8_rows_kernel<float, float, float, false><<<rows, threads, 0, s>>>((float*)x, nullptr, nullptr, nullptr, (signed char*)values, scales, x_stride, rows, k, stride, 0.f);
-    else
-        int8_rows_kernel<bf16, float, float, false><<<rows, threads, 0, s>>>((bf16*)x, nullptr, nullptr, nullptr, (signed char*)values, scales, x_stride, rows, k, stride, 0.f);
+#define XRT_ROWS8(TX, PIECES) int8_rows_kernel<TX, float, float, false, PIECES><<<rows, threads_for(stride, PIECES), 0, s>>>((TX*)x, nullptr, nullptr, nullptr, (signed char*)values, scales, x_stride, rows, k, stride, 0.f)
+    // two pieces a thread up to 8192 columns, four beyond: more of a wide row is then in flight (bfloat16, 8192 rows of 14336: 104 us with one, 78 with two,
+    // 67 with four, 73 with eight; 2048 of 8192: 19.0, 11.1, 11.8 and 11.6; 8192 of 513: 8.9, 5.9, 7.0 and 10.4)
+    if (dtype == XRT_F32 && stride <= 8192) XRT_ROWS8(float, 2);
+    else if (dtype == XRT_F32) XRT_ROWS8(float, 4);
+    else if (stride <= 8192) XRT_ROWS8(bf16, 2);
+    else XRT_ROWS8(bf16, 4);
+#undef XRT_ROWS8
     XRT_LAUNCH_CHECK("quantize_int8");
     return 0;
 }
@@ -229,13 +248,21 @@ extern "C" int xrt_rmsnorm_int8(float* x, const void* delta, int delta_dtype, co
     XRT_REQUIRE(!delta || !rows, "rmsnorm_int8: chosen rows of x cannot be added to (one might be chosen twice)");
     XRT_REQUIRE(rows || n_rows == x_rows, "rmsnorm_int8: %d rows of results for %d rows of x", n_rows, x_rows);
     if (n_rows == 0) return 0;
-    const int stride = (int)int8_stride(hidden), threads = threads_for(stride);
+    const int stride = (int)int8_stride(hidden);
     hipStream_t s = (hipStream_t)stream;
-#define XRT_NORM8(TD, TW) int8_rows_kernel<float, TD, TW, true><<<n_rows, threads, 0, s>>>(x, (const TD*)delta, (const TW*)weight, rows, (signed char*)values, scales, hidden, x_rows, hidden, stride, eps)
-    if (delta_dtype == XRT_BF16 && weight_dtype == XRT_BF16) XRT_NORM8(bf16, bf16);
-    else if (delta_dtype == XRT_BF16) XRT_NORM8(bf16, float);
-    else if (weight_dtype == XRT_BF16) XRT_NORM8(float, bf16);
-    else XRT_NORM8(float, float);
+#define XRT_NORM8(TD, TW, PIECES) int8_rows_kernel<float, TD, TW, true, PIECES><<<n_rows, threads_for(stride, PIECES), 0, s>>>(x, (const TD*)delta, (const TW*)weight, rows, (signed char*)values, scales, hidden, x_rows, hidden, stride, eps)
+#define XRT_NORM8_OF(PIECES)                                                                      \
+    do {                                                                                          \
+        if (delta_dtype == XRT_BF16 && weight_dtype == XRT_BF16) XRT_NORM8(bf16, bf16, PIECES);   \
+        else if (delta_dtype == XRT_BF16) XRT_NORM8(bf16, float, PIECES);                         \
+        else if (weight_dtype == XRT_BF16) XRT_NORM8(float, bf16, PIECES);                        \
+        else XRT_NORM8(float, float, PIECES);                                                     \
+    } while (0)
+    // two pieces a thread, with the gains in registers ahead of the sum (8 rows of 4096 4.4 us, 4.8 with one piece, 5.3 with four and the gains fetched behind
+    // the sum; 333 of 5120 7.9, 9.5 and 8.4; 16384 of 4096 163 us with either, 4.5 TB/s)
+    if (stride <= 2 * 8 * MOST_THREADS) XRT_NORM8_OF(2);
+    else XRT_NORM8_OF(4);
+#undef XRT_NORM8_OF
 #undef XRT_NORM8
     XRT_LAUNCH_CHECK("rmsnorm_int8");
     return 0;
@@ -245,11 +272,12 @@ extern "C" int xrt_dequantize_int8(const void* values, const float* scales, void
     XRT_REQUIRE(rows >= 0 && k > 0 && k <= XRT_INT8_MOST_K && (rows == 0 || (values && scales && out)), "dequantize_int8: bad operands rows=%d k=%d", rows, k);
     XRT_REQUIRE(out_dtype == XRT_F32 || out_dtype == XRT_BF16, "dequantize_int8: unknown dtype %d", out_dtype);
     if (rows == 0) return 0;
-    const long blocks = ((long)rows * ((k + 7) / 8) + 255) / 256;
-    XRT_REQUIRE(blocks < (1L << 31), "dequantize_int8: too many elements");
+    int lanes = 8;
+    while (lanes < 256 && lanes * 8 < k) lanes *= 2;
+    const dim3 blocks((unsigned)((rows + (long)(256 / lanes) - 1) / (256 / lanes)), (unsigned)((k + lanes * 8 - 1) / (lanes * 8)));
     hipStream_t s = (hipStream_t)stream;
-    if (out_dtype == XRT_F32) int8_values_kernel<float><<<(unsigned)blocks, 256, 0, s>>>((const signed char*)values, scales, (float*)out, rows, k, (int)int8_stride(k));
-    else int8_values_kernel<bf16><<<(unsigned)blocks, 256, 0, s>>>((const signed char*)values, scales, (bf16*)out, rows, k, (int)int8_stride(k));
+    if (out_dtype == XRT_F32) int8_values_kernel<float><<<blocks, 256, 0, s>>>((const signed char*)values, scales, (float*)out, rows, k, (int)int8_stride(k), lanes);
+    else int8_values_kernel<bf16><<<blocks, 256, 0, s>>>((const signed char*)values, scales, (bf16*)out, rows, k, (int)int8_stride(k), lanes);
     XRT_LAUNCH_CHECK("dequantize_int8");
     return 0;
 }

@@ -18,6 +18,7 @@ _CODES = {torch.float32: 0, torch.bfloat16: 1}
 
 # the handle of the current stream of a device (by its index)
 _raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None) or (lambda index: torch.cuda.current_stream(index).cuda_stream)
+_current_device = getattr(torch._C, "_cuda_getDevice", None) or torch.cuda.current_device
 
 
 class KernelError(RuntimeError):
@@ -116,30 +117,45 @@ INT8_MOST_K = 131071        # columns of which a sum of products still fits 32 b
 class Int8Rows:
     """Rows in 8-bit integers: row m stands for values[m, :k] * scales[m]. values is int8 [rows, k filled up to a multiple of INT8_STEP], with zeros
     behind the k columns; scales float32 [rows]. `int8_rows` makes an empty one; `quantize_int8` and `rmsnorm_int8` fill it, `linear_int8` and
-    `linear_glu_int8` multiply it. Whoever fills one in another way keeps the zeros."""
+    `linear_glu_int8` multiply it. Whoever fills one in another way keeps the zeros. The tensors are checked here, once, and stay what they are."""
 
-    __slots__ = ("values", "scales", "k")
+    __slots__ = ("_values", "_scales", "_k", "shape", "index")
 
     def __init__(self, values: torch.Tensor, scales: torch.Tensor, k: int):
-        self.values, self.scales, self.k = values, scales, int(k)
+        rows, k = values.shape[0] if values.dim() == 2 else -1, int(k)
+        if not 0 < k <= INT8_MOST_K:
+            raise KernelError(f"rows in 8 bits: {k} columns, expected 1 to {INT8_MOST_K}")
+        HipOps._require(values, "8-bit values", torch.int8, (rows, (k + INT8_STEP - 1) // INT8_STEP * INT8_STEP))
+        HipOps._require(scales, "scales of 8-bit rows", torch.float32, (rows,), values)
+        if values.data_ptr() % 16 != 0:                         # (they are read sixteen bytes at a time)
+            raise KernelError("8-bit values must start at a multiple of 16 bytes")
+        self._values, self._scales, self._k, self.shape, self.index = values, scales, k, (rows, k), values.get_device()
 
     @property
-    def shape(self):
-        return (self.values.shape[0], self.k)
+    def values(self) -> torch.Tensor:
+        return self._values
+
+    @property
+    def scales(self) -> torch.Tensor:
+        return self._scales
+
+    @property
+    def k(self) -> int:
+        return self._k
 
     @property
     def device(self):
-        return self.values.device
+        return self._values.device
 
 
 class Int8Matrix:
     """A weight matrix [rows, k] in 8-bit integers with a scale for each row (output channel), in the tiles in which the products take it
     (csrc/int8.h). gated: [gate rows | up rows], for `linear_glu_int8`. Made by `pack_int8`."""
 
-    __slots__ = ("data", "scales", "shape", "gated")
+    __slots__ = ("data", "scales", "shape", "gated", "index")
 
     def __init__(self, data: torch.Tensor, scales: torch.Tensor, rows: int, k: int, gated: bool):
-        self.data, self.scales, self.shape, self.gated = data, scales, (rows, k), gated
+        self.data, self.scales, self.shape, self.gated, self.index = data, scales, (rows, k), gated, data.get_device()
 
     @property
     def device(self):
@@ -299,6 +315,14 @@ class HipOps:
         self.lib.xrt_experts_sort_room.restype = ctypes.c_long
         self.lib.xrt_attention_latent_workspace.restype = ctypes.c_long
         self.lib.xrt_linear_int8_workspace.restype = ctypes.c_long
+        # (calls whose arguments are declared take plain numbers: addresses need no object each. Two microseconds of eight a call.)
+        at, whole, long, real = ctypes.c_void_p, ctypes.c_int, ctypes.c_long, ctypes.c_float
+        self.lib.xrt_quantize_int8.argtypes = [at, whole, long, at, at, whole, whole, at]
+        self.lib.xrt_rmsnorm_int8.argtypes = [at, at, whole, at, whole, real, at, at, at, whole, whole, whole, at]
+        self.lib.xrt_dequantize_int8.argtypes = [at, at, at, whole, whole, whole, at]
+        self.lib.xrt_pack_int8.argtypes = [at, at, at, at, whole, whole, whole, at]
+        self.lib.xrt_linear_int8.argtypes = [at, at, at, at, at, whole, whole, whole, whole, whole, at, long, at]
+        self.lib.xrt_linear_int8_workspace.argtypes = [whole, whole, whole, whole]
 
     # -- helpers -------------------------------------------------------------
     def _check(self, status: int) -> None:
@@ -574,24 +598,22 @@ class HipOps:
         self._linear(a, w_gate_up, out, 2 | (ACTIVATIONS[activation] << 8), w_gate_up.shape[0] // 2)
 
     # -- rows and weights in 8-bit integers --------------------------------------
+    # (A decode step makes four of these calls a layer, of a few microseconds each on the GPU: what is checked is checked once a call, and in few steps.)
     @staticmethod
-    def _on_current_device(tensor) -> None:
-        """The kernels start on the current device: tensors of another one are refused."""
-        if tensor.get_device() != torch.cuda.current_device():
-            raise KernelError(f"the tensors are on {tensor.device}, the current device is cuda:{torch.cuda.current_device()}")
+    def _int8_stream(index: int) -> int:
+        """The handle of the current stream of device `index`, which has to be the current device: the kernels start there."""
+        if index != _current_device():
+            raise KernelError(f"the tensors are on cuda:{index}, the current device is cuda:{_current_device()}")
+        return _raw_stream(index)
 
-    def _require_int8(self, rows, what: str, shape, like=None) -> None:
+    @staticmethod
+    def _is_int8(rows, what: str, shape, index: int) -> None:
         if not isinstance(rows, Int8Rows):
             raise KernelError(f"{what}: expected Int8Rows")
-        if rows.shape != tuple(shape):
+        if rows.shape != shape:
             raise KernelError(f"{what}: rows of shape {rows.shape}, expected {tuple(shape)}")
-        count, k = shape
-        if not 0 < k <= INT8_MOST_K:
-            raise KernelError(f"{what}: rows of {k} columns, expected 1 to {INT8_MOST_K}")
-        self._require(rows.values, f"{what} values", torch.int8, (count, (k + INT8_STEP - 1) // INT8_STEP * INT8_STEP), like)
-        self._require(rows.scales, f"{what} scales", torch.float32, (count,), rows.values)
-        if rows.values.data_ptr() % 16 != 0:                    # (they are read sixteen bytes at a time)
-            raise KernelError(f"{what}: values must start at a multiple of 16 bytes")
+        if rows.index != index:
+            raise KernelError(f"{what}: on cuda:{rows.index}, expected cuda:{index}")
 
     def int8_rows(self, rows: int, k: int, device) -> Int8Rows:
         """Room for `rows` rows of k columns in 8-bit integers; what it holds is not defined."""
@@ -603,12 +625,10 @@ class HipOps:
     def quantize_int8(self, x, out: Int8Rows):
         """out = the rows of x (float32 or bfloat16, some columns of a wider matrix will do) in 8-bit integers: scales[m] = max |x[m]| / 127, values =
         x / scale rounded to the nearest integer, halves to even. A row of zeros has scale 0; one that holds an infinity or a NaN scale NaN and zeros."""
-        stride = self._rows(x, "quantize_int8 x")
-        code = _code(x)
-        self._require_int8(out, "quantize_int8 out", x.shape, x)
-        self._on_current_device(x)
-        self._check(self.lib.xrt_quantize_int8(_ptr(x), code, ctypes.c_long(stride), _ptr(out.values), _ptr(out.scales), x.shape[0], x.shape[1],
-                                               self._stream(x)))
+        stride, index = self._rows(x, "quantize_int8 x"), x.get_device()
+        self._is_int8(out, "quantize_int8 out", x.shape, index)
+        rows, k = out.shape
+        self._check(self.lib.xrt_quantize_int8(x.data_ptr(), _code(x), stride, out._values.data_ptr(), out._scales.data_ptr(), rows, k, self._int8_stream(index)))
 
     def rmsnorm_int8(self, x, weight, eps, out: Int8Rows, delta=None, rows=None):
         """x += delta in place, if given (float32 or bfloat16, shaped like x), then out = the rows x / sqrt(mean(x^2) + eps) * weight as `quantize_int8`
@@ -619,7 +639,7 @@ class HipOps:
             raise KernelError("rmsnorm_int8 x: expected [rows, hidden]")
         x_rows, hidden = x.shape
         self._require(weight, "rmsnorm_int8 weight", None, (hidden,), x)
-        count = x_rows
+        count, at_rows, at_delta, delta_code = x_rows, None, None, 0
         if rows is not None:
             if delta is not None:
                 raise KernelError("rmsnorm_int8: chosen rows of x cannot be added to (one might be chosen twice)")
@@ -627,71 +647,71 @@ class HipOps:
                 raise KernelError("rmsnorm_int8 rows: expected a list of rows on the GPU")
             count = rows.shape[0]
             self._require(rows, "rmsnorm_int8 rows", torch.int32, (count,), x)
-        if delta is not None:
-            self._require(delta, "rmsnorm_int8 delta", None, (x_rows, hidden), x)
-        self._require_int8(out, "rmsnorm_int8 out", (count, hidden), x)
-        self._on_current_device(x)
-        self._check(self.lib.xrt_rmsnorm_int8(_ptr(x), _ptr(delta), 0 if delta is None else _code(delta), _ptr(weight), _code(weight), ctypes.c_float(eps),
-                                              _ptr(out.values), _ptr(out.scales), _ptr(rows), count, x_rows, hidden, self._stream(x)))
+            at_rows = rows.data_ptr()
+        elif delta is not None:
+            self._require(delta, "rmsnorm_int8 delta", None, x.shape, x)
+            at_delta, delta_code = delta.data_ptr(), _code(delta)
+        index = x.get_device()
+        self._is_int8(out, "rmsnorm_int8 out", (count, hidden), index)
+        self._check(self.lib.xrt_rmsnorm_int8(x.data_ptr(), at_delta, delta_code, weight.data_ptr(), _code(weight), eps, out._values.data_ptr(),
+                                              out._scales.data_ptr(), at_rows, count, x_rows, hidden, self._int8_stream(index)))
 
     def dequantize_int8(self, rows: Int8Rows, out):
         """out[m, j] = values[m, j] * scales[m] (float32 or bfloat16)."""
-        self._require_int8(rows, "dequantize_int8 rows", rows.shape)
-        self._require(out, "dequantize_int8 out", None, rows.shape, rows.values)
-        self._on_current_device(out)
-        self._check(self.lib.xrt_dequantize_int8(_ptr(rows.values), _ptr(rows.scales), _ptr(out), _code(out), rows.shape[0], rows.k, self._stream(out)))
+        if not isinstance(rows, Int8Rows):
+            raise KernelError("dequantize_int8 rows: expected Int8Rows")
+        self._require(out, "dequantize_int8 out", None, rows.shape, rows._values)
+        count, k = rows.shape
+        self._check(self.lib.xrt_dequantize_int8(rows._values.data_ptr(), rows._scales.data_ptr(), out.data_ptr(), _code(out), count, k,
+                                                 self._int8_stream(rows.index)))
 
     def pack_int8(self, w, gated: bool = False) -> Int8Matrix:
         """The weight matrix w [rows, k] for `linear_int8`, or gated ([gate rows | up rows]) for `linear_glu_int8`: Int8Rows, or a float matrix, whose
         rows (output channels) are then brought to 8 bits as `quantize_int8` does it."""
         if not isinstance(w, Int8Rows):
-            if not isinstance(w, torch.Tensor) or w.dim() != 2 or 0 in w.shape:
-                raise KernelError("pack_int8: w must be [rows, k]")
+            if not isinstance(w, torch.Tensor) or not w.is_cuda or w.dim() != 2 or 0 in w.shape:
+                raise KernelError("pack_int8: w must be [rows, k], on the GPU")
             as_rows = self.int8_rows(w.shape[0], w.shape[1], w.device)
             self.quantize_int8(w, as_rows)
             w = as_rows
         rows, k = w.shape
         if rows < 1 or (gated and rows % 2 != 0):
             raise KernelError(f"pack_int8: {rows} rows; a gated matrix has gate rows followed by as many up rows")
-        self._require_int8(w, "pack_int8 w", w.shape)
-        self._on_current_device(w.values)
         n = rows // 2 if gated else rows
         packed_rows = (n + 7) // 8 * 16 if gated else (n + 15) // 16 * 16
         data = torch.empty(packed_rows, w.values.shape[1], dtype=torch.int8, device=w.device)
         scales = torch.empty(packed_rows, dtype=torch.float32, device=w.device)
-        self._check(self.lib.xrt_pack_int8(_ptr(w.values), _ptr(w.scales), _ptr(data), _ptr(scales), n, k, int(gated), self._stream(data)))
+        self._check(self.lib.xrt_pack_int8(w.values.data_ptr(), w.scales.data_ptr(), data.data_ptr(), scales.data_ptr(), n, k, int(gated),
+                                           self._int8_stream(w.index)))
         return Int8Matrix(data, scales, rows, k, bool(gated))
 
     def _linear_int8(self, a, w, out, mode, n):
-        if not isinstance(w, Int8Matrix):
-            raise KernelError("linear_int8 w: expected an Int8Matrix")
-        rows, k = w.shape
+        k, index = w.shape[1], w.index
+        if not isinstance(a, Int8Rows):
+            raise KernelError("8-bit product: a must be Int8Rows")
         m = a.shape[0]
-        self._require_int8(a, "linear_int8 a", (m, k), w.data)
-        self._require(out, "linear_int8 out", None, (m, n), w.data)
-        if mode == 1 and out.dtype != torch.float32:
+        self._is_int8(a, "8-bit product a", (m, k), index)
+        self._require(out, "8-bit product out", None, (m, n), w.data)
+        code = _code(out)
+        if mode == 1 and code != 0:
             raise KernelError(f"linear_int8 out: added to in {out.dtype}, expected float32")
-        self._on_current_device(out)
-        need = int(self.lib.xrt_linear_int8_workspace(m, n, k, mode))
+        stream = self._int8_stream(index)
+        need = self.lib.xrt_linear_int8_workspace(m, n, k, mode)
         workspace = self._empty(need // 4, torch.int32, out.device) if need > 0 else None
-        self._check(self.lib.xrt_linear_int8(_ptr(a.values), _ptr(a.scales), _ptr(w.data), _ptr(w.scales), _ptr(out), _code(out), m, n, k, mode,
-                                             _ptr(workspace), ctypes.c_long(need), self._stream(out)))
+        self._check(self.lib.xrt_linear_int8(a._values.data_ptr(), a._scales.data_ptr(), w.data.data_ptr(), w.scales.data_ptr(), out.data_ptr(), code, m, n, k, mode,
+                                             None if workspace is None else workspace.data_ptr(), need, stream))
 
     def linear_int8(self, a: Int8Rows, w: Int8Matrix, out, accumulate=False):
         """out[m, n] (+)= (sum over j of a[m, j] w[n, j], exact) * a.scales[m] * w.scales[n], in float32; out is float32 or bfloat16, float32 if it is
         added to. A row's result has the same bits whatever the other rows are."""
-        if isinstance(w, Int8Matrix) and w.gated:
-            raise KernelError("linear_int8 w: packed for linear_glu_int8")
-        if not isinstance(a, Int8Rows):
-            raise KernelError("linear_int8 a: expected Int8Rows")
+        if not isinstance(w, Int8Matrix) or w.gated:
+            raise KernelError("linear_int8 w: expected an Int8Matrix that is not gated")
         self._linear_int8(a, w, out, 1 if accumulate else 0, w.shape[0])
 
     def linear_glu_int8(self, a: Int8Rows, w_gate_up: Int8Matrix, out, activation: str = "silu"):
         """out = act(gate) * up of the two products with w_gate_up = [gate rows | up rows], each as `linear_int8` makes it."""
-        if isinstance(w_gate_up, Int8Matrix) and not w_gate_up.gated:
-            raise KernelError("linear_glu_int8 w: packed for linear_int8")
-        if not isinstance(a, Int8Rows):
-            raise KernelError("linear_glu_int8 a: expected Int8Rows")
+        if not isinstance(w_gate_up, Int8Matrix) or not w_gate_up.gated:
+            raise KernelError("linear_glu_int8 w: expected a gated Int8Matrix")
         if activation not in ACTIVATIONS:
             raise KernelError(f"linear_glu_int8: activation must be one of {sorted(ACTIVATIONS)}, found {activation!r}")
         self._linear_int8(a, w_gate_up, out, 2 | (ACTIVATIONS[activation] << 8), w_gate_up.shape[0] // 2)
