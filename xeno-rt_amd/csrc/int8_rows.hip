@@ -24,9 +24,9 @@ __device__ __forceinline__ void load_eight(const T* row, int at, int width, floa
         for (int e = 0; e < 8; ++e) v[e] = at + e < width ? to_float(row[at + e]) : 0.f;
     }
 }
-// past_caches: nobody reads the row again before it would have left them.
+// The same on the way back. (16384 rows of 4096 normed, with the sums written: 148 us; 163 where the compiler was left to find the pieces in a copy of the array.)
 template <typename T>
-__device__ __forceinline__ void store_eight(T* row, int at, int width, const float (&v)[8], bool past_caches) {
+__device__ __forceinline__ void store_eight(T* row, int at, int width, const float (&v)[8]) {
     typedef unsigned Words __attribute__((ext_vector_type(4)));
     typedef Words Anywhere __attribute__((aligned(2)));                // (in memory: aligned as the smallest element is)
     Eight<T> piece;
@@ -37,9 +37,7 @@ __device__ __forceinline__ void store_eight(T* row, int at, int width, const flo
         for (int h = 0; h < (int)sizeof(T) / 2; ++h) {
             Words part;
             __builtin_memcpy(&part, piece.e + h * (16 / sizeof(T)), 16);
-            Anywhere* to = reinterpret_cast<Anywhere*>(row + at) + h;
-            if (past_caches) __builtin_nontemporal_store(part, to);
-            else *to = part;
+            reinterpret_cast<Anywhere*>(row + at)[h] = part;
         }
     } else {
 #pragma unroll
@@ -47,9 +45,6 @@ __device__ __forceinline__ void store_eight(T* row, int at, int width, const flo
             if (at + e < width) row[at + e] = piece.e[e];
     }
 }
-// Whether so many bytes are written past the caches: what is larger than half of the last one (256 MB) has mostly left it when it is read again.
-// (16384 rows of 4096 normed with the sum written back 163 -> 149 us; 2048 rows, whose sums stay, take 18.8 either way and are left to be found there.)
-bool goes_past_caches(long bytes) { return bytes > (128L << 20); }
 
 // The bits of |v|: as whole numbers they are ordered as the magnitudes are, infinity above all numbers and NaN above infinity.
 __device__ __forceinline__ unsigned magnitude_bits(float v) { return __builtin_bit_cast(unsigned, v) & 0x7fffffffu; }
@@ -104,7 +99,7 @@ constexpr int MOST_THREADS = 1024;
 template <typename TX, typename TD, typename TW, bool NORM, int PIECES>
 __global__ void __launch_bounds__(MOST_THREADS) int8_rows_kernel(TX* x, const TD* delta, const TW* __restrict__ weight, const int* __restrict__ rows,
                                                                  signed char* __restrict__ values, float* __restrict__ scales, long x_stride,
-                                                                 int x_rows, int width, int stride, float eps, bool past_caches) {
+                                                                 int x_rows, int width, int stride, float eps) {
     __shared__ float sums[32];
     __shared__ unsigned maxima[16];
     const long r = blockIdx.x;
@@ -133,7 +128,7 @@ __global__ void __launch_bounds__(MOST_THREADS) int8_rows_kernel(TX* x, const TD
             load_eight(add, at, width, d);
 #pragma unroll
             for (int e = 0; e < 8; ++e) v[e] += d[e];
-            store_eight(row, at, width, v, past_caches);
+            store_eight(row, at, width, v);
         };
         float sum = 0.f;
 #pragma unroll
@@ -194,7 +189,7 @@ __global__ void __launch_bounds__(MOST_THREADS) int8_rows_kernel(TX* x, const TD
 // out[m][j] = values[m][j] * scales[m]: `lanes` threads a row (a power of two up to 256), a thread eight neighbouring columns
 template <typename TO>
 __global__ void __launch_bounds__(256) int8_values_kernel(const signed char* __restrict__ values, const float* __restrict__ scales, TO* __restrict__ out,
-                                                          int rows, int width, int stride, int lanes, unsigned chunks, bool past_caches) {
+                                                          int rows, int width, int stride, int lanes, unsigned chunks) {
     const long r = (long)(blockIdx.x / chunks) * (256 / lanes) + threadIdx.x / lanes;
     const int at = ((int)(blockIdx.x % chunks) * lanes + (int)threadIdx.x % lanes) * 8;
     if (r >= rows || at >= width) return;
@@ -203,7 +198,7 @@ __global__ void __launch_bounds__(256) int8_values_kernel(const signed char* __r
     float v[8];
 #pragma unroll
     for (int e = 0; e < 8; ++e) v[e] = (float)(int)(signed char)((e < 4 ? bytes.x : bytes.y) >> (e % 4 * 8)) * scale;
-    store_eight(out + r * width, at, width, v, past_caches);
+    store_eight(out + r * width, at, width, v);
 }
 
 // A thread a 16-byte piece of the packed matrix; the threads of the first tile of a group see to its scales.
@@ -240,7 +235,7 @@ extern "C" int xrt_quantize_int8(const void* x, int dtype, long x_stride, void* 
     if (rows == 0) return 0;
     const int stride = (int)int8_stride(k);
     hipStream_t s = (hipStream_t)stream;
-#define XRT_ROWS8(TX, PIECES) int8_rows_kernel<TX, float, float, false, PIECES><<<rows, threads_for(stride, PIECES), 0, s>>>((TX*)x, nullptr, nullptr, nullptr, (signed char*)values, scales, x_stride, rows, k, stride, 0.f, false)
+#define XRT_ROWS8(TX, PIECES) int8_rows_kernel<TX, float, float, false, PIECES><<<rows, threads_for(stride, PIECES), 0, s>>>((TX*)x, nullptr, nullptr, nullptr, (signed char*)values, scales, x_stride, rows, k, stride, 0.f)
     // two pieces a thread up to 8192 columns, four beyond: more of a wide row is then in flight (bfloat16, 8192 rows of 14336: 104 us with one, 78 with two,
     // 67 with four, 73 with eight; 2048 of 8192: 19.0, 11.1, 11.8 and 11.6; 8192 of 513: 8.9, 5.9, 7.0 and 10.4)
     if (dtype == XRT_F32 && stride <= 8192) XRT_ROWS8(float, 2);
@@ -262,9 +257,8 @@ extern "C" int xrt_rmsnorm_int8(float* x, const void* delta, int delta_dtype, co
     XRT_REQUIRE(rows || n_rows == x_rows, "rmsnorm_int8: %d rows of results for %d rows of x", n_rows, x_rows);
     if (n_rows == 0) return 0;
     const int stride = (int)int8_stride(hidden);
-    const bool past_caches = goes_past_caches((long)x_rows * hidden * (long)sizeof(float));
     hipStream_t s = (hipStream_t)stream;
-#define XRT_NORM8(TD, TW, PIECES) int8_rows_kernel<float, TD, TW, true, PIECES><<<n_rows, threads_for(stride, PIECES), 0, s>>>(x, (const TD*)delta, (const TW*)weight, rows, (signed char*)values, scales, hidden, x_rows, hidden, stride, eps, past_caches)
+#define XRT_NORM8(TD, TW, PIECES) int8_rows_kernel<float, TD, TW, true, PIECES><<<n_rows, threads_for(stride, PIECES), 0, s>>>(x, (const TD*)delta, (const TW*)weight, rows, (signed char*)values, scales, hidden, x_rows, hidden, stride, eps)
 #define XRT_NORM8_OF(PIECES)                                                                      \
     do {                                                                                          \
         if (delta_dtype == XRT_BF16 && weight_dtype == XRT_BF16) XRT_NORM8(bf16, bf16, PIECES);   \
@@ -290,10 +284,9 @@ extern "C" int xrt_dequantize_int8(const void* values, const float* scales, void
     while (lanes < 256 && lanes * 8 < k) lanes *= 2;
     const long chunks = (k + lanes * 8 - 1) / (lanes * 8), blocks = (rows + (long)(256 / lanes) - 1) / (256 / lanes) * chunks;
     XRT_REQUIRE(blocks < (1L << 31), "dequantize_int8: too many elements");
-    const bool past_caches = goes_past_caches((long)rows * k * (out_dtype == XRT_F32 ? 4 : 2));
     hipStream_t s = (hipStream_t)stream;
-    if (out_dtype == XRT_F32) int8_values_kernel<float><<<(unsigned)blocks, 256, 0, s>>>((const signed char*)values, scales, (float*)out, rows, k, (int)int8_stride(k), lanes, (unsigned)chunks, past_caches);
-    else int8_values_kernel<bf16><<<(unsigned)blocks, 256, 0, s>>>((const signed char*)values, scales, (bf16*)out, rows, k, (int)int8_stride(k), lanes, (unsigned)chunks, past_caches);
+    if (out_dtype == XRT_F32) int8_values_kernel<float><<<(unsigned)blocks, 256, 0, s>>>((const signed char*)values, scales, (float*)out, rows, k, (int)int8_stride(k), lanes, (unsigned)chunks);
+    else int8_values_kernel<bf16><<<(unsigned)blocks, 256, 0, s>>>((const signed char*)values, scales, (bf16*)out, rows, k, (int)int8_stride(k), lanes, (unsigned)chunks);
     XRT_LAUNCH_CHECK("dequantize_int8");
     return 0;
 }
