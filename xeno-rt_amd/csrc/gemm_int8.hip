@@ -21,6 +21,44 @@ namespace {
 typedef int int4v __attribute__((ext_vector_type(4)));
 enum { MODE_STORE = 0, MODE_ACCUMULATE = 1, MODE_GATED = 2 };
 
+// Neighbouring columns of a row of out [M][N], in one piece wherever they lie (global memory wants no more than an element's alignment), and those that
+// are there where the row ends inside the piece. (Four accesses of one element each instead: 1588 rows added to, 717 channels, k = 384 21.7 us, 13.9 so.)
+template <typename T, int COUNT> struct Run { T e[COUNT]; };
+template <typename TO>
+__device__ __forceinline__ void load_run(const TO* out, long m, long n, int M, int N, float (&v)[4]) {
+    const TO* row = out + min(m, (long)M - 1) * (long)N;       // (rows and columns beyond the matrix: something inside, not used)
+    if (n + 4 <= N) {
+        Run<TO, 4> run;
+        __builtin_memcpy(&run, row + n, sizeof(run));
+#pragma unroll
+        for (int e = 0; e < 4; ++e) v[e] = to_float(run.e[e]);
+    } else {
+#pragma unroll
+        for (int e = 0; e < 4; ++e) v[e] = to_float(row[min(n + e, (long)N - 1)]);
+    }
+}
+template <typename TO, int COUNT>
+__device__ __forceinline__ void store_run(TO* out, long m, long n, int M, int N, const Run<TO, COUNT>& run) {
+    typedef unsigned Words __attribute__((ext_vector_type(COUNT * sizeof(TO) / 4)));
+    typedef Words Anywhere __attribute__((aligned(2)));
+    if (m >= M || n >= N) return;
+    TO* row = out + m * (long)N + n;
+    if (n + COUNT <= N) {
+        *reinterpret_cast<Anywhere*>(row) = __builtin_bit_cast(Words, run);
+    } else {
+#pragma unroll
+        for (int e = 0; e < COUNT; ++e)
+            if (n + e < N) row[e] = run.e[e];
+    }
+}
+template <typename TO>
+__device__ __forceinline__ void store_run(TO* out, long m, long n, int M, int N, const float (&v)[4]) {
+    Run<TO, 4> run;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) run.e[e] = from_float<TO>(v[e]);
+    store_run<TO, 4>(out, m, n, M, N, run);
+}
+
 __device__ __forceinline__ float scaled(int sum, float a_scale, float w_scale) { return (float)sum * a_scale * w_scale; }
 
 // What a product writes, and what the sums are multiplied by.
@@ -53,14 +91,13 @@ __device__ __forceinline__ void finish_block(const int4v sum, long m0, long grou
         mine = mine && c < 2;
     }
     if (!mine || n >= to.N) return;
-    const bool wide = to.N % 4 == 0 && (uintptr_t)to.out % 16 == 0;
     if constexpr (MODE == MODE_ACCUMULATE) {
         float before[4];
-        load_four<TO>(to.out, m, n, to.M, to.N, before, wide);
+        load_run<TO>(to.out, m, n, to.M, to.N, before);
 #pragma unroll
         for (int e = 0; e < 4; ++e) value[e] = before[e] + value[e];
     }
-    store_four<TO>(to.out, m, n, to.M, to.N, value, wide);
+    store_run<TO>(to.out, m, n, to.M, to.N, value);
 }
 
 // Adds the parts of every block, one wavefront a block: sums[part][16 rows of a][group][lane].
@@ -79,22 +116,28 @@ __global__ void __launch_bounds__(256) int8_finish_kernel(const int4v* __restric
 
 constexpr int WAVES = 8;
 
-// MT: blocks of 16 rows of a (all of them); G: groups of 16 packed rows of w a workgroup. Its wavefronts share out k, each with a run of its own, and add
-// their sums through LDS. Nothing is read twice by a workgroup, so a's rows come from L2 as often as there are workgroups: with G groups a workgroup reads
-// MT / G times as much of a as of w. PARTS: k is cut among blockIdx.y.
-template <int MT, int G, int MODE, typename TO, bool PARTS>
+// MT: blocks of 16 rows of a; G: groups of 16 packed rows of w a workgroup. Its wavefronts share out k, each with a run of its own, and add their sums
+// through LDS. Nothing is read twice by a workgroup, so a's rows come from L2 as often as there are workgroups along n: with G groups a workgroup reads
+// MT / G times as much of a as of w. PARTS: k is cut among workgroups. ONCE: the rows of a are one tile, so that every byte of w is read by one workgroup,
+// and is asked for past the caches.
+template <int MT, int G, int MODE, typename TO, bool PARTS, bool ONCE>
 __global__ void __launch_bounds__(WAVES * XRT_WAVE, MT * G <= 2 ? 4 : 2) gemm_int8_few_kernel(const signed char* __restrict__ a, const signed char* __restrict__ w,
-                                                                                          int4v* __restrict__ sums, int M, int stride, int groups, int parts,
-                                                                                          const Result<TO> to) {
+                                                                                          int4v* __restrict__ sums, int M, int stride, int groups, int tiles_m,
+                                                                                          int tiles_n, int parts, const Result<TO> to) {
     constexpr int AT_ONCE = G * MT < 8 ? G * MT : 8;            // blocks whose sums lie in LDS at one time
     __shared__ int4v shared[WAVES][AT_ONCE][XRT_WAVE];
+    // An XCD gets a run of tiles; split over one tile of rows: tiles and parts in turn. (8 rows, k = 4096, 1792 groups 20.4 us in runs, 23.2 in turn; 64 rows,
+    // k = 14336, 4096 channels in four parts 19.4 and 17.8.)
+    const PartPlace place = PARTS && ONCE ? PartPlace{TilePlace{(int)blockIdx.x < tiles_n * parts ? 0 : -1, (int)blockIdx.x % tiles_n}, (int)blockIdx.x / tiles_n}
+                                          : part_place(blockIdx.x, 0, tiles_m, tiles_n, PARTS ? parts : 0);
+    if (place.tile.m < 0) return;
     const int lane = threadIdx.x % XRT_WAVE, wave = __builtin_amdgcn_readfirstlane(threadIdx.x / XRT_WAVE);
     const int r = lane % 16, c = lane / 16;
-    const int first_group = blockIdx.x * G;
+    const int first_group = place.tile.n * G, first_block = place.tile.m * MT;
 
     // units of 128 columns, dealt evenly to the parts and within a part to the wavefronts
     const int units = stride / XRT_INT8_STEP;
-    const int part = PARTS ? blockIdx.y : 0;
+    const int part = PARTS ? place.part : 0;
     const int begin = PARTS ? (int)((long)units * part / parts) : 0, end = PARTS ? (int)((long)units * (part + 1) / parts) : units;
     const int first = begin + (end - begin) * wave / WAVES, count = begin + (end - begin) * (wave + 1) / WAVES - first;
 
@@ -103,7 +146,7 @@ __global__ void __launch_bounds__(WAVES * XRT_WAVE, MT * G <= 2 ? 4 : 2) gemm_in
 #pragma unroll
     for (int g = 0; g < G; ++g) w_at[g] = w + (long)min(first_group + g, groups - 1) * 16 * stride + (long)first * 2048 + lane * 16;       // groups beyond the matrix: the last one again
 #pragma unroll
-    for (int i = 0; i < MT; ++i) a_at[i] = a + (long)min(i * 16 + r, M - 1) * stride + (long)first * 128 + c * 16;                         // rows likewise
+    for (int i = 0; i < MT; ++i) a_at[i] = a + (long)min((first_block + i) * 16 + r, M - 1) * stride + (long)first * 128 + c * 16;         // rows likewise
 
     struct Unit { int4v w[G][2], a[MT][2]; };
     auto load = [&](Unit& unit, int u) {
@@ -114,7 +157,10 @@ __global__ void __launch_bounds__(WAVES * XRT_WAVE, MT * G <= 2 ? 4 : 2) gemm_in
 #pragma unroll
         for (int g = 0; g < G; ++g)
 #pragma unroll
-            for (int j = 0; j < 2; ++j) unit.w[g][j] = __builtin_nontemporal_load(reinterpret_cast<const int4v*>(w_at[g] + (long)u * 2048 + j * 1024));
+            for (int j = 0; j < 2; ++j) {
+                const int4v* from = reinterpret_cast<const int4v*>(w_at[g] + (long)u * 2048 + j * 1024);
+                unit.w[g][j] = ONCE ? __builtin_nontemporal_load(from) : *from;
+            }
     };
     int4v acc[G][MT];
 #pragma unroll
@@ -129,8 +175,9 @@ __global__ void __launch_bounds__(WAVES * XRT_WAVE, MT * G <= 2 ? 4 : 2) gemm_in
 #pragma unroll
                 for (int i = 0; i < MT; ++i) acc[g][i] = __builtin_amdgcn_mfma_i32_16x16x64_i8(unit.w[g][j], unit.a[i][j], acc[g][i], 0, 0, 0);
     };
-    // a ring of units: while one is multiplied the others are on their way
-    constexpr int RING = G * MT >= 16 ? 2 : G * MT >= 4 ? 3 : 4;
+    // Two units in turn: while one is multiplied the other is on its way. (Three or four cost the workgroups that run beside this one their registers:
+    // 32 rows, k = 4096, 14336 pairs 30.1 us with three, 27.7 with two.)
+    constexpr int RING = 2;
     Unit ring[RING];
 #pragma unroll
     for (int b = 0; b < RING; ++b)
@@ -163,10 +210,10 @@ __global__ void __launch_bounds__(WAVES * XRT_WAVE, MT * G <= 2 ? 4 : 2) gemm_in
         int4v sum = shared[0][wave][lane];
 #pragma unroll
         for (int other = 1; other < WAVES; ++other) sum += shared[other][wave][lane];
-        const int group = first_group + (t0 + wave) / MT, block = (t0 + wave) % MT;
+        const int group = first_group + (t0 + wave) / MT, block = first_block + (t0 + wave) % MT;
         if (group >= groups || block * 16 >= M) continue;
         if constexpr (PARTS) sums[(((long)part * ((M + 15) / 16) + block) * groups + group) * XRT_WAVE + lane] = sum;
-        else finish_block<MODE, TO>(sum, block * 16, group, to);
+        else finish_block<MODE, TO>(sum, (long)block * 16, group, to);
     }
 }
 
@@ -366,13 +413,13 @@ __global__ void __launch_bounds__(8 * XRT_WAVE) gemm_int8_large_kernel(const sig
         return scaled(acc[i][j][e], a_scale[i], of_channel);
     };
     TO* out = to.out;
+    typedef Run<TO, 8> Eight;
     if constexpr (MODE == MODE_GATED) {
         // A group of 16 packed rows holds the gate rows of 8 outputs, then their up rows: the lane with an output's up sum
         // is 32 lanes away. One exchange of half a register between the sums of two blocks of a leaves gate and up of
         // every output of both in one lane (lanes 0 to 31 the first block's outputs, the others the second's); for
         // bfloat16 another one between two groups of w brings eight neighbouring outputs together: 16 bytes a store.
         const long n_wave = (long)wave_group * 8;
-        const bool wide = N % 8 == 0 && (uintptr_t)out % 16 == 0;
 #pragma unroll
         for (int i = 0; i < TM; i += 2) {
             const long m = wave_row + lane % 16 + i * 16 + lane / 32 * 16;
@@ -388,51 +435,41 @@ __global__ void __launch_bounds__(8 * XRT_WAVE) gemm_int8_large_kernel(const sig
                         made[u][e] = gate_activation<sizeof(TO) == 2>(gate, to.activation) * up;
                     }
                 if constexpr (sizeof(TO) == 2) {
-                    if (wide) {
-                        const uint4v piece = join_rows<TO>(made[0], made[1]);
-                        const long n = n_wave + (j + quad % 2) * 8;
-                        if (m < row_end && n < N) *reinterpret_cast<uint4v*>(out + m * (long)N + n) = piece;
-                        continue;
-                    }
-                }
+                    store_run<TO, 8>(out, m, n_wave + (j + quad % 2) * 8, row_end, N, __builtin_bit_cast(Eight, join_rows<TO>(made[0], made[1])));
+                } else {
 #pragma unroll
-                for (int u = 0; u < 2; ++u) store_four<TO>(out, m, n_wave + (j + u) * 8 + quad % 2 * 4, row_end, N, made[u], wide);
+                    for (int u = 0; u < 2; ++u) store_run<TO>(out, m, n_wave + (j + u) * 8 + quad % 2 * 4, row_end, N, made[u]);
+                }
             }
         }
     } else {
-        const bool wide = N % 8 == 0 && (uintptr_t)out % 16 == 0;
         // Two neighbouring blocks of columns change eight lanes with each other, so that an instruction takes eight rows of
         // 128 bytes, whole cache lines, instead of sixteen of 64.
         const long row8 = wave_row + lane % 8;
         const int upper = lane % 16 / 8;
         if constexpr (MODE == MODE_STORE && sizeof(TO) == 2) {
-            if (wide) {
-                static_assert(TN == 4, "two pieces of 32 columns");
-                const long n = (long)wave_group * 16 + (2 * upper + quad % 2) * 16 + quad / 2 * 8;
+            static_assert(TN == 4, "two pieces of 32 columns");
+            const long n = (long)wave_group * 16 + (2 * upper + quad % 2) * 16 + quad / 2 * 8;
 #pragma unroll
-                for (int i = 0; i < TM; ++i) {
-                    uint4v piece[2];
+            for (int i = 0; i < TM; ++i) {
+                uint4v piece[2];
 #pragma unroll
-                    for (int u = 0; u < 2; ++u) {
-                        const float first[4] = {value(i, 2 * u, 0), value(i, 2 * u, 1), value(i, 2 * u, 2), value(i, 2 * u, 3)};
-                        const float second[4] = {value(i, 2 * u + 1, 0), value(i, 2 * u + 1, 1), value(i, 2 * u + 1, 2), value(i, 2 * u + 1, 3)};
-                        piece[u] = join_rows<TO>(first, second);
-                    }
-#pragma unroll
-                    for (int e = 0; e < 4; ++e) {
-                        unsigned low = piece[0][e], high = piece[1][e];
-                        exchange_eights(low, high);
-                        piece[0][e] = low;
-                        piece[1][e] = high;
-                    }
-#pragma unroll
-                    for (int u = 0; u < 2; ++u) {
-                        const long m = row8 + i * 16 + u * 8;
-                        if (m < row_end && n < N) *reinterpret_cast<uint4v*>(out + m * (long)N + n) = piece[u];
-                    }
+                for (int u = 0; u < 2; ++u) {
+                    const float first[4] = {value(i, 2 * u, 0), value(i, 2 * u, 1), value(i, 2 * u, 2), value(i, 2 * u, 3)};
+                    const float second[4] = {value(i, 2 * u + 1, 0), value(i, 2 * u + 1, 1), value(i, 2 * u + 1, 2), value(i, 2 * u + 1, 3)};
+                    piece[u] = join_rows<TO>(first, second);
                 }
-                return;
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    unsigned low = piece[0][e], high = piece[1][e];
+                    exchange_eights(low, high);
+                    piece[0][e] = low;
+                    piece[1][e] = high;
+                }
+#pragma unroll
+                for (int u = 0; u < 2; ++u) store_run<TO, 8>(out, row8 + i * 16 + u * 8, n, row_end, N, __builtin_bit_cast(Eight, piece[u]));
             }
+            return;
         }
         constexpr int RUN = TM % 4 == 0 ? 4 : 3;               // blocks of a whose old values are read in one go, before any is written
 #pragma unroll
@@ -443,7 +480,7 @@ __global__ void __launch_bounds__(8 * XRT_WAVE) gemm_int8_large_kernel(const sig
                 for (int i = 0; i < RUN; ++i)
 #pragma unroll
                     for (int j = 0; j < TN; ++j)
-                        load_four<TO>(out, row8 + (i0 + i) * 16 + j % 2 * 8, (long)(wave_group + j / 2 * 2 + upper) * 16 + quad * 4, row_end, N, before[i][j], wide);
+                        load_run<TO>(out, row8 + (i0 + i) * 16 + j % 2 * 8, (long)(wave_group + j / 2 * 2 + upper) * 16 + quad * 4, row_end, N, before[i][j]);
             }
 #pragma unroll
             for (int i = 0; i < RUN; ++i)
@@ -461,8 +498,8 @@ __global__ void __launch_bounds__(8 * XRT_WAVE) gemm_int8_large_kernel(const sig
                         }
                     }
                     const long n = (long)(wave_group + j + upper) * 16 + quad * 4;
-                    store_four<TO>(out, row8 + (i0 + i) * 16, n, row_end, N, made[0], wide);
-                    store_four<TO>(out, row8 + (i0 + i) * 16 + 8, n, row_end, N, made[1], wide);
+                    store_run<TO>(out, row8 + (i0 + i) * 16, n, row_end, N, made[0]);
+                    store_run<TO>(out, row8 + (i0 + i) * 16 + 8, n, row_end, N, made[1]);
                 }
         }
     }
@@ -479,24 +516,33 @@ struct Plan {
 
 Plan plan_of(long M, long groups, long stride) {
     const long units = stride / XRT_INT8_STEP;
-    if (M <= 64) {
-        const int blocks = M <= 16 ? 1 : M <= 32 ? 2 : 4;
-        Plan plan{0, blocks, blocks, 1};
-        const long workgroups = (groups + plan.groups - 1) / plan.groups;
-        while (plan.parts < 8 && workgroups * plan.parts * 2 <= (blocks == 1 ? XRT_COMPUTE_UNITS / 2 : XRT_COMPUTE_UNITS) && units / (plan.parts * 2) >= 8) plan.parts *= 2;
-        return plan;
+    // The kernel of few rows: up to 64, and more where its tiles of 64 x 64 find a compute unit each and no workgroup goes through more than 7168 columns (a
+    // tile reads as much of a as of w). It takes a half to nine tenths of the time of the larger tiles there (217 rows, k = 384, 1312 channels 6.9 -> 4.5 us;
+    // 447, 1536, 1440 14.0 -> 7.6; 456, 7168, 912 pairs 23.7 -> 21.0; 239, 7552, 1496 pairs 20.9 -> 22.7).
+    {
+        // (two blocks of rows, 1792 groups of w: 27.7 us with two groups a workgroup, 24.5 with four; 384 groups: 9.5 and 11.1)
+        Plan plan{0, M <= 16 ? 1 : M <= 32 ? 2 : 4, M <= 16 ? 1 : M <= 32 && groups < 4 * XRT_COMPUTE_UNITS ? 2 : 4, 1};
+        const long workgroups = (M + plan.blocks * 16 - 1) / (plan.blocks * 16) * ((groups + plan.groups - 1) / plan.groups);
+        const long most = plan.blocks == 1 ? XRT_COMPUTE_UNITS / 2 : XRT_COMPUTE_UNITS;
+        while (plan.parts < 8 && workgroups * plan.parts * 2 <= most && units / (plan.parts * 2) >= 4) plan.parts *= 2;
+        if (M <= 64 || (workgroups <= XRT_COMPUTE_UNITS && units <= plan.parts * 56)) return plan;
     }
+    // What a tile height costs, fitted to products of 4096 rows, k = 4096 and 14336 (us): a step along k (256 rows: 1.31, 128: 0.80), and the first loads and the
+    // epilogue. A partly filled round takes half of a full one and its share of the rest: power bounds the chip, and the compute units at work run faster.
     Plan plan{0, 0, 0, 1};
     const long tiles_n = (groups + 15) / 16;
     double best = 0;
     for (const int tile : {256, 192, 128}) {
+        const int height = even_height((int)M, tile);
         const long tiles = (M + tile - 1) / tile * tiles_n;
-        const long rounds = (tiles + XRT_COMPUTE_UNITS - 1) / XRT_COMPUTE_UNITS;
-        const double cost = rounds * (even_height((int)M, tile) + 32.0);
+        const double rest = (double)(tiles % XRT_COMPUTE_UNITS) / XRT_COMPUTE_UNITS;
+        const double cost = (tiles / XRT_COMPUTE_UNITS + (rest > 0 ? 0.55 + 0.45 * rest : 0)) * (units * (height + 73) * 0.004 + 2.7 + 0.0234 * tile);
         if (plan.tile == 0 || cost < best) plan.tile = tile, best = cost;
     }
     const long tiles = (M + plan.tile - 1) / plan.tile * tiles_n;
-    while (plan.parts < 16 && tiles * plan.parts * 2 <= XRT_COMPUTE_UNITS && units / (plan.parts * 2) >= 4) plan.parts *= 2;
+    while (plan.parts < 16 && tiles * plan.parts * 2 <= XRT_COMPUTE_UNITS && units / (plan.parts * 2) >= 3) plan.parts *= 2;
+    const long steps = (units + plan.parts - 1) / plan.parts;
+    plan.parts = (int)((units + steps - 1) / steps);           // (none is empty)
     return plan;
 }
 
@@ -504,11 +550,14 @@ long sums_bytes(const Plan& plan, long M, long groups) { return plan.parts == 1 
 
 struct Operands { const signed char* a; const signed char* w; int4v* sums; int stride, groups; hipStream_t stream; };
 
-template <int MT, int G, int MODE, typename TO>
-void launch_few(const Operands& o, const Plan& plan, const Result<TO>& to) {
-    const dim3 grid((o.groups + G - 1) / G, plan.parts);
-    if (plan.parts == 1) gemm_int8_few_kernel<MT, G, MODE, TO, false><<<grid, WAVES * XRT_WAVE, 0, o.stream>>>(o.a, o.w, nullptr, to.M, o.stride, o.groups, 1, to);
-    else gemm_int8_few_kernel<MT, G, MODE_STORE, float, true><<<grid, WAVES * XRT_WAVE, 0, o.stream>>>(o.a, o.w, o.sums, to.M, o.stride, o.groups, plan.parts, Result<float>{});
+template <int MT, int G, int MODE, typename TO, bool ONCE = true>
+int launch_few(const Operands& o, const Plan& plan, const Result<TO>& to) {
+    const int tiles_m = (to.M + MT * 16 - 1) / (MT * 16), tiles_n = (o.groups + G - 1) / G;
+    const long ids = part_ids((long)tiles_m * tiles_n, plan.parts, true);        // a whole number of rounds over the XCDs
+    XRT_REQUIRE(ids < (1L << 31), "linear_int8: %ld tiles", ids);
+    if (plan.parts == 1) gemm_int8_few_kernel<MT, G, MODE, TO, false, ONCE><<<(unsigned)ids, WAVES * XRT_WAVE, 0, o.stream>>>(o.a, o.w, nullptr, to.M, o.stride, o.groups, tiles_m, tiles_n, 1, to);
+    else gemm_int8_few_kernel<MT, G, MODE_STORE, float, true, ONCE><<<(unsigned)ids, WAVES * XRT_WAVE, 0, o.stream>>>(o.a, o.w, o.sums, to.M, o.stride, o.groups, tiles_m, tiles_n, plan.parts, Result<float>{});
+    return 0;
 }
 
 template <int BM, int MODE, typename TO, bool PARTS>
@@ -535,12 +584,11 @@ template <int MODE, typename TO>
 int launch(const Operands& o, const Plan& plan, const Result<TO>& to) {
     int failed = 0;
     if (plan.tile == 0) {
-        const int kind = plan.blocks * 8 + plan.groups;
-        if (kind == 8 + 1) launch_few<1, 1, MODE, TO>(o, plan, to);
-        else if (kind == 16 + 1) launch_few<2, 1, MODE, TO>(o, plan, to);
-        else if (kind == 16 + 2) launch_few<2, 2, MODE, TO>(o, plan, to);
-        else if (kind == 32 + 1) launch_few<4, 1, MODE, TO>(o, plan, to);
-        else launch_few<4, 4, MODE, TO>(o, plan, to);
+        if (plan.blocks == 1) failed = launch_few<1, 1, MODE, TO>(o, plan, to);
+        else if (plan.blocks == 2 && plan.groups == 2) failed = launch_few<2, 2, MODE, TO>(o, plan, to);
+        else if (plan.blocks == 2) failed = launch_few<2, 4, MODE, TO>(o, plan, to);
+        else if (to.M <= 64) failed = launch_few<4, 4, MODE, TO>(o, plan, to);
+        else failed = launch_few<4, 4, MODE, TO, false>(o, plan, to);
     } else if (plan.parts > 1) {
         Result<float> sizes{};
         sizes.M = to.M, sizes.N = to.N;

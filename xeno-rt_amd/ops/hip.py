@@ -615,6 +615,14 @@ class HipOps:
         if rows.index != index:
             raise KernelError(f"{what}: on cuda:{rows.index}, expected cuda:{index}")
 
+    def _is_tensor(self, tensor, what: str, dtype, shape, index: int) -> int:
+        """The address of a contiguous tensor of that type (None: any), shape and device; anything else is refused."""
+        if not (isinstance(tensor, torch.Tensor) and (dtype is None or tensor.dtype is dtype) and tensor.shape == shape and tensor.is_contiguous()
+                and tensor.get_device() == index):
+            self._require(tensor, what, dtype, shape)
+            raise KernelError(f"{what}: on {tensor.device}, expected cuda:{index}")
+        return tensor.data_ptr()
+
     def int8_rows(self, rows: int, k: int, device) -> Int8Rows:
         """Room for `rows` rows of k columns in 8-bit integers; what it holds is not defined."""
         if rows < 0 or not 0 < k <= INT8_MOST_K:
@@ -637,8 +645,8 @@ class HipOps:
         self._require(x, "rmsnorm_int8 x", torch.float32)
         if x.dim() != 2:
             raise KernelError("rmsnorm_int8 x: expected [rows, hidden]")
-        x_rows, hidden = x.shape
-        self._require(weight, "rmsnorm_int8 weight", None, (hidden,), x)
+        (x_rows, hidden), index = x.shape, x.get_device()
+        at_weight = self._is_tensor(weight, "rmsnorm_int8 weight", None, (hidden,), index)
         count, at_rows, at_delta, delta_code = x_rows, None, None, 0
         if rows is not None:
             if delta is not None:
@@ -646,24 +654,20 @@ class HipOps:
             if not isinstance(rows, torch.Tensor) or rows.dim() != 1:
                 raise KernelError("rmsnorm_int8 rows: expected a list of rows on the GPU")
             count = rows.shape[0]
-            self._require(rows, "rmsnorm_int8 rows", torch.int32, (count,), x)
-            at_rows = rows.data_ptr()
+            at_rows = self._is_tensor(rows, "rmsnorm_int8 rows", torch.int32, (count,), index)
         elif delta is not None:
-            self._require(delta, "rmsnorm_int8 delta", None, x.shape, x)
-            at_delta, delta_code = delta.data_ptr(), _code(delta)
-        index = x.get_device()
+            at_delta, delta_code = self._is_tensor(delta, "rmsnorm_int8 delta", None, x.shape, index), _code(delta)
         self._is_int8(out, "rmsnorm_int8 out", (count, hidden), index)
-        self._check(self.lib.xrt_rmsnorm_int8(x.data_ptr(), at_delta, delta_code, weight.data_ptr(), _code(weight), eps, out._values.data_ptr(),
-                                              out._scales.data_ptr(), at_rows, count, x_rows, hidden, self._int8_stream(index)))
+        self._check(self.lib.xrt_rmsnorm_int8(x.data_ptr(), at_delta, delta_code, at_weight, _code(weight), eps, out._values.data_ptr(), out._scales.data_ptr(),
+                                              at_rows, count, x_rows, hidden, self._int8_stream(index)))
 
     def dequantize_int8(self, rows: Int8Rows, out):
         """out[m, j] = values[m, j] * scales[m] (float32 or bfloat16)."""
         if not isinstance(rows, Int8Rows):
             raise KernelError("dequantize_int8 rows: expected Int8Rows")
-        self._require(out, "dequantize_int8 out", None, rows.shape, rows._values)
-        count, k = rows.shape
-        self._check(self.lib.xrt_dequantize_int8(rows._values.data_ptr(), rows._scales.data_ptr(), out.data_ptr(), _code(out), count, k,
-                                                 self._int8_stream(rows.index)))
+        (count, k), index = rows.shape, rows.index
+        at_out = self._is_tensor(out, "dequantize_int8 out", None, rows.shape, index)
+        self._check(self.lib.xrt_dequantize_int8(rows._values.data_ptr(), rows._scales.data_ptr(), at_out, _code(out), count, k, self._int8_stream(index)))
 
     def pack_int8(self, w, gated: bool = False) -> Int8Matrix:
         """The weight matrix w [rows, k] for `linear_int8`, or gated ([gate rows | up rows]) for `linear_glu_int8`: Int8Rows, or a float matrix, whose
@@ -691,14 +695,13 @@ class HipOps:
             raise KernelError("8-bit product: a must be Int8Rows")
         m = a.shape[0]
         self._is_int8(a, "8-bit product a", (m, k), index)
-        self._require(out, "8-bit product out", None, (m, n), w.data)
-        code = _code(out)
+        at_out, code = self._is_tensor(out, "8-bit product out", None, (m, n), index), _code(out)
         if mode == 1 and code != 0:
             raise KernelError(f"linear_int8 out: added to in {out.dtype}, expected float32")
         stream = self._int8_stream(index)
         need = self.lib.xrt_linear_int8_workspace(m, n, k, mode)
         workspace = self._empty(need // 4, torch.int32, out.device) if need > 0 else None
-        self._check(self.lib.xrt_linear_int8(a._values.data_ptr(), a._scales.data_ptr(), w.data.data_ptr(), w.scales.data_ptr(), out.data_ptr(), code, m, n, k, mode,
+        self._check(self.lib.xrt_linear_int8(a._values.data_ptr(), a._scales.data_ptr(), w.data.data_ptr(), w.scales.data_ptr(), at_out, code, m, n, k, mode,
                                              None if workspace is None else workspace.data_ptr(), need, stream))
 
     def linear_int8(self, a: Int8Rows, w: Int8Matrix, out, accumulate=False):
