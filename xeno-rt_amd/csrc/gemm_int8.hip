@@ -219,18 +219,16 @@ __global__ void __launch_bounds__(WAVES * XRT_WAVE, MT * G <= 2 ? 4 : 2) gemm_in
 
 // ---- more rows --------------------------------------------------------------------------------------------------------------------------------------------
 
-constexpr int BN = 256;                // packed rows of w in a tile
-
-// Tiles of BM (256, 192 or 128) rows of a by 256 packed rows of w: eight wavefronts, two to a SIMD, which take turns as those of the bfloat16 product's large
+// Tiles of BM (256, 192 or 128) rows of a by BN (256, or 128) packed rows of w: eight wavefronts, two to a SIMD, which take turns as those of the bfloat16 product's large
 // tiles do. Of the two on a SIMD (one of each group of four) one reads the operands of its next products from LDS and asks for tiles to come while the other
-// multiplies; a barrier ends a turn, and the second group runs one barrier behind the first. A wavefront's part (BM / 2 x 64) is four quarters along k: (half
+// multiplies; a barrier ends a turn, and the second group runs one barrier behind the first. A wavefront's part (BM / 2 x BN / 4) is four quarters along k: (half
 // h of its rows of a, half g of its rows of w) in the order (0,0) (0,1) (1,1) (1,0), so that every turn reads one new half: w0, w1, a1, and a0 of the next
 // tile. A half is loaded into the place of the same half two tiles ago as soon as both groups have read that, seven quarters before it is needed, and the
 // waits leave the newer six quarters' loads in flight.
 //
 // height: the rows of a that a tile stands for, a multiple of 16 up to BM (even_height): the first four wavefronts take half of the blocks of 16, or one
 // more than the others, and a wavefront runs the loop made for its number of blocks (all, one or two fewer).
-template <int BM, int MODE, typename TO, bool PARTS>
+template <int BM, int BN, int MODE, typename TO, bool PARTS>
 __global__ void __launch_bounds__(8 * XRT_WAVE) gemm_int8_large_kernel(const signed char* __restrict__ a, const signed char* __restrict__ w, int4v* __restrict__ sums,
                                                                        int stride, int groups, int tiles_m, int tiles_n, int height, int by_parts,
                                                                        int steps_a_part, const Result<TO> to) {
@@ -243,7 +241,7 @@ __global__ void __launch_bounds__(8 * XRT_WAVE) gemm_int8_large_kernel(const sig
     unsigned char* stage_a = lds_raw;                          // [2][BM][128]: rows of eight 16-byte pieces, swizzled
     unsigned char* stage_b = stage_a + 2 * BM * STEP;          // [2][16 groups][2][1024]: packed tiles as they lie
     float* lds_a_scales = reinterpret_cast<float*>(stage_b + 2 * BN * STEP);      // [256] of the tile's rows
-    float* lds_w_scales = lds_a_scales + 256;                  // [256]
+    float* lds_w_scales = lds_a_scales + 256;                  // [BN]
 
     const PartPlace dealt = PARTS ? part_place(blockIdx.x, blockIdx.y, tiles_m, tiles_n, by_parts) : PartPlace{tile_place(blockIdx.x, tiles_m, tiles_n), 0};
     if (dealt.tile.m < 0) return;
@@ -296,7 +294,7 @@ __global__ void __launch_bounds__(8 * XRT_WAVE) gemm_int8_large_kernel(const sig
     // the tile's scales, ahead of the tiles themselves: wavefronts 0 to 3 those of 64 rows of a each, 4 to 7 those of 64 packed rows of w
     if constexpr (!PARTS) {
         if (wave < 4) load_dword_to_lds(to.a_scales, (unsigned)min(m0 + wave * 64 + lane, M - 1) * 4u, lds_address(lds_a_scales + wave * 64));
-        else load_dword_to_lds(to.w_scales, (unsigned)min(first_group * 16 + (wave - 4) * 64 + lane, groups * 16 - 1) * 4u, lds_address(lds_w_scales + (wave - 4) * 64));
+        else if ((wave - 4) * 64 < BN) load_dword_to_lds(to.w_scales, (unsigned)min(first_group * 16 + (wave - 4) * 64 + lane, groups * 16 - 1) * 4u, lds_address(lds_w_scales + (wave - 4) * 64));
     }
     // where this lane finds its 16 bytes of block 0 of its wavefront, for either 64 columns of the tile
     const unsigned char* place_a[2];
@@ -448,6 +446,16 @@ __global__ void __launch_bounds__(8 * XRT_WAVE) gemm_int8_large_kernel(const sig
         const long row8 = wave_row + lane % 8;
         const int upper = lane % 16 / 8;
         if constexpr (MODE == MODE_STORE && sizeof(TO) == 2) {
+            if constexpr (TN == 2) {                           // (one piece of 32 columns: sixteen rows of 64 bytes)
+#pragma unroll
+                for (int i = 0; i < TM; ++i) {
+                    const float first[4] = {value(i, 0, 0), value(i, 0, 1), value(i, 0, 2), value(i, 0, 3)};
+                    const float second[4] = {value(i, 1, 0), value(i, 1, 1), value(i, 1, 2), value(i, 1, 3)};
+                    store_run<TO, 8>(out, wave_row + i * 16 + lane % 16, (long)wave_group * 16 + quad % 2 * 16 + quad / 2 * 8, row_end, N,
+                                     __builtin_bit_cast(Eight, join_rows<TO>(first, second)));
+                }
+                return;
+            } else {
             static_assert(TN == 4, "two pieces of 32 columns");
             const long n = (long)wave_group * 16 + (2 * upper + quad % 2) * 16 + quad / 2 * 8;
 #pragma unroll
@@ -470,6 +478,7 @@ __global__ void __launch_bounds__(8 * XRT_WAVE) gemm_int8_large_kernel(const sig
                 for (int u = 0; u < 2; ++u) store_run<TO, 8>(out, row8 + i * 16 + u * 8, n, row_end, N, __builtin_bit_cast(Eight, piece[u]));
             }
             return;
+            }
         }
         constexpr int RUN = TM % 4 == 0 ? 4 : 3;               // blocks of a whose old values are read in one go, before any is written
 #pragma unroll
@@ -509,6 +518,7 @@ __global__ void __launch_bounds__(8 * XRT_WAVE) gemm_int8_large_kernel(const sig
 
 struct Plan {
     int tile;           // rows of a of a tile (256, 192, 128), or 0: the kernel of few rows
+    int width;          // packed rows of w of a tile (256 or 128)
     int blocks;         // of 16 rows of a, of the kernel of few rows (1, 2 or 4)
     int groups;         // of w a workgroup, of the same (1, 2 or 4)
     int parts;          // of k
@@ -521,7 +531,7 @@ Plan plan_of(long M, long groups, long stride) {
     // 447, 1536, 1440 14.0 -> 7.6; 456, 7168, 912 pairs 23.7 -> 21.0; 239, 7552, 1496 pairs 20.9 -> 22.7).
     {
         // (two blocks of rows, 1792 groups of w: 27.7 us with two groups a workgroup, 24.5 with four; 384 groups: 9.5 and 11.1)
-        Plan plan{0, M <= 16 ? 1 : M <= 32 ? 2 : 4, M <= 16 ? 1 : M <= 32 && groups < 4 * XRT_COMPUTE_UNITS ? 2 : 4, 1};
+        Plan plan{0, 0, M <= 16 ? 1 : M <= 32 ? 2 : 4, M <= 16 ? 1 : M <= 32 && groups < 4 * XRT_COMPUTE_UNITS ? 2 : 4, 1};
         const long workgroups = (M + plan.blocks * 16 - 1) / (plan.blocks * 16) * ((groups + plan.groups - 1) / plan.groups);
         const long most = plan.blocks == 1 ? XRT_COMPUTE_UNITS / 2 : XRT_COMPUTE_UNITS;
         while (plan.parts < 8 && workgroups * plan.parts * 2 <= most && units / (plan.parts * 2) >= 4) plan.parts *= 2;
@@ -529,7 +539,7 @@ Plan plan_of(long M, long groups, long stride) {
     }
     // What a tile height costs, fitted to products of 4096 rows, k = 4096 and 14336 (us): a step along k (256 rows: 1.31, 128: 0.80), and the first loads and the
     // epilogue. A partly filled round takes half of a full one and its share of the rest: power bounds the chip, and the compute units at work run faster.
-    Plan plan{0, 0, 0, 1};
+    Plan plan{0, 256, 0, 0, 1};
     const long tiles_n = (groups + 15) / 16;
     double best = 0;
     for (const int tile : {256, 192, 128}) {
@@ -539,7 +549,9 @@ Plan plan_of(long M, long groups, long stride) {
         const double cost = (tiles / XRT_COMPUTE_UNITS + (rest > 0 ? 0.55 + 0.45 * rest : 0)) * (units * (height + 73) * 0.004 + 2.7 + 0.0234 * tile);
         if (plan.tile == 0 || cost < best) plan.tile = tile, best = cost;
     }
-    const long tiles = (M + plan.tile - 1) / plan.tile * tiles_n;
+    long tiles = (M + plan.tile - 1) / plan.tile * tiles_n;
+    // Tiles half as wide where the others fill up to half of the chip: a compute unit has a limit of its own on what it has asked for of w.
+    if (plan.tile == 128 && tiles * 2 <= XRT_COMPUTE_UNITS) plan.width = 128, tiles = (M + 127) / 128 * ((groups + 7) / 8);
     while (plan.parts < 16 && tiles * plan.parts * 2 <= XRT_COMPUTE_UNITS && units / (plan.parts * 2) >= 3) plan.parts *= 2;
     const long steps = (units + plan.parts - 1) / plan.parts;
     plan.parts = (int)((units + steps - 1) / steps);           // (none is empty)
@@ -560,10 +572,10 @@ int launch_few(const Operands& o, const Plan& plan, const Result<TO>& to) {
     return 0;
 }
 
-template <int BM, int MODE, typename TO, bool PARTS>
+template <int BM, int BN, int MODE, typename TO, bool PARTS>
 int launch_large(const Operands& o, const Plan& plan, const Result<TO>& to) {
     constexpr size_t lds = (size_t)2 * (BM + BN) * XRT_INT8_STEP + 2 * 256 * sizeof(float);
-    auto kernel = gemm_int8_large_kernel<BM, MODE, TO, PARTS>;
+    auto kernel = gemm_int8_large_kernel<BM, BN, MODE, TO, PARTS>;
     static bool configured[64] = {};                           // per instantiation and device
     int device = 0;
     XRT_REQUIRE(hipGetDevice(&device) == hipSuccess, "linear_int8: no current device");
@@ -573,7 +585,7 @@ int launch_large(const Operands& o, const Plan& plan, const Result<TO>& to) {
         if (device >= 0 && device < 64) configured[device] = true;
     }
     const int units = o.stride / XRT_INT8_STEP, steps = (units + plan.parts - 1) / plan.parts;
-    const int height = even_height(to.M, BM), tiles_m = (to.M + height - 1) / height, tiles_n = (o.groups + 15) / 16;
+    const int height = even_height(to.M, BM), tiles_m = (to.M + height - 1) / height, tiles_n = (o.groups + BN / 16 - 1) / (BN / 16);
     const long ids = part_ids((long)tiles_m * tiles_n, plan.parts, true);        // a whole number of rounds over the XCDs
     XRT_REQUIRE(ids < (1L << 31), "linear_int8: %ld tiles", ids);
     kernel<<<(unsigned)ids, 8 * XRT_WAVE, lds, o.stream>>>(o.a, o.w, o.sums, o.stride, o.groups, tiles_m, tiles_n, height, plan.parts, steps, to);
@@ -592,12 +604,14 @@ int launch(const Operands& o, const Plan& plan, const Result<TO>& to) {
     } else if (plan.parts > 1) {
         Result<float> sizes{};
         sizes.M = to.M, sizes.N = to.N;
-        if (plan.tile == 256) failed = launch_large<256, MODE_STORE, float, true>(o, plan, sizes);
-        else if (plan.tile == 192) failed = launch_large<192, MODE_STORE, float, true>(o, plan, sizes);
-        else failed = launch_large<128, MODE_STORE, float, true>(o, plan, sizes);
-    } else if (plan.tile == 256) failed = launch_large<256, MODE, TO, false>(o, plan, to);
-    else if (plan.tile == 192) failed = launch_large<192, MODE, TO, false>(o, plan, to);
-    else failed = launch_large<128, MODE, TO, false>(o, plan, to);
+        if (plan.tile == 256) failed = launch_large<256, 256, MODE_STORE, float, true>(o, plan, sizes);
+        else if (plan.tile == 192) failed = launch_large<192, 256, MODE_STORE, float, true>(o, plan, sizes);
+        else if (plan.width == 256) failed = launch_large<128, 256, MODE_STORE, float, true>(o, plan, sizes);
+        else failed = launch_large<128, 128, MODE_STORE, float, true>(o, plan, sizes);
+    } else if (plan.tile == 256) failed = launch_large<256, 256, MODE, TO, false>(o, plan, to);
+    else if (plan.tile == 192) failed = launch_large<192, 256, MODE, TO, false>(o, plan, to);
+    else if (plan.width == 256) failed = launch_large<128, 256, MODE, TO, false>(o, plan, to);
+    else failed = launch_large<128, 128, MODE, TO, false>(o, plan, to);
     if (failed) return failed;
     if (plan.parts > 1) {
         const long blocks = (long)((to.M + 15) / 16) * o.groups;
