@@ -48,52 +48,6 @@ class EmulatedOps:
             self.values, self.squares, self.eps = values, squares, eps
             self.shape = values.shape
 
-    # -- rows and weights in 8-bit integers ---------------------------------------
-    class Int8Rows:
-        def __init__(self, rows, k):
-            self.shape, self.values, self.scales = (rows, k), None, None
-
-    class Int8Matrix:
-        def __init__(self, rows, gated):
-            self.values, self.scales, self.shape, self.gated = rows.values, rows.scales, rows.shape, gated
-
-    def int8_rows(self, rows, k, device):
-        return self.Int8Rows(rows, k)
-
-    def quantize_int8(self, x, out):
-        x = x.to(torch.float32)
-        assert tuple(x.shape) == out.shape
-        most = x.abs().amax(1)
-        out.scales = most / torch.full_like(most, 127.0)
-        out.values = torch.where(out.scales[:, None] > 0, x / out.scales[:, None], torch.zeros_like(x)).round().clamp(-127, 127)
-        broken = ~torch.isfinite(x).all(1)
-        out.scales[broken], out.values[broken] = float("nan"), 0.0
-
-    def rmsnorm_int8(self, x, weight, eps, out, delta=None, rows=None):
-        if delta is not None:
-            x.add_(delta.to(torch.float32))
-        y = torch.empty(out.shape, device=x.device)
-        self.rmsnorm(x, weight, eps, y, rows=rows)
-        self.quantize_int8(y, out)
-
-    def dequantize_int8(self, rows, out):
-        out.copy_(rows.values * rows.scales[:, None])
-
-    def pack_int8(self, w, gated=False):
-        if not isinstance(w, self.Int8Rows):
-            rows = self.Int8Rows(*w.shape)
-            self.quantize_int8(w, rows)
-            w = rows
-        return self.Int8Matrix(w, gated)
-
-    def _int8_product(self, a, w):
-        if not isinstance(a, self.Int8Rows):
-            rows = self.Int8Rows(*a.shape)
-            self.quantize_int8(a, rows)
-            a = rows
-        sums = (a.values.double() @ w.values.double().t()).to(torch.float32)      # whole numbers: exact, then rounded once
-        return sums * a.scales[:, None] * w.scales
-
     def _rows(self, a):
         if isinstance(a, self.Prescaled):
             inv = 1.0 / torch.sqrt(a.squares / a.values.shape[-1] + a.eps)
@@ -101,11 +55,6 @@ class EmulatedOps:
         return a.to(torch.float32), 1.0
 
     def linear(self, a, w, out, accumulate=False, then_norm=None):
-        if isinstance(w, self.Int8Matrix):
-            assert not w.gated
-            result = self._int8_product(a, w)
-            out.copy_((out.to(torch.float32) + result if accumulate else result).to(out.dtype))
-            return None
         rows, inv = self._rows(a)
         result = (rows @ w.to(torch.float32).t()) * inv
         if accumulate:
@@ -121,12 +70,8 @@ class EmulatedOps:
     def linear_glu(self, a, w_gate_up, out, activation="silu"):
         assert activation == "silu"
         inter = w_gate_up.shape[0] // 2
-        if isinstance(w_gate_up, self.Int8Matrix):
-            assert w_gate_up.gated
-            both = self._int8_product(a, w_gate_up)
-        else:
-            rows, inv = self._rows(a)
-            both = (rows @ w_gate_up.to(torch.float32).t()) * inv
+        rows, inv = self._rows(a)
+        both = (rows @ w_gate_up.to(torch.float32).t()) * inv
         gate, up = both[:, :inter], both[:, inter:]
         out.copy_(((gate / (1.0 + torch.exp(-gate))) * up).to(out.dtype))
 

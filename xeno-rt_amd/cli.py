@@ -41,7 +41,6 @@ def build_parser() -> argparse.ArgumentParser:
     gen.add_argument("--seed", type=int, default=None)
     gen.add_argument("--stop-ids", default=None, help="stop token ids, e.g. 2,5 (default: eos_token_id of config.json)")
     gen.add_argument("--dtype", default="bfloat16", choices=["bfloat16", "float32", "bf16", "fp32"])
-    gen.add_argument("--int8-weights", action="store_true", help="keep the layers' matrices in 8-bit integers, with a scale for each output channel")
     gen.add_argument("--batch-size", type=int, default=None, help="most requests that run together")
     gen.add_argument("--cache-tokens", type=int, default=None, help="tokens the cache holds (default: what the batch needs)")
     write = commands.add_parser("random-model", help="write a model folder with random weights")
@@ -66,11 +65,11 @@ def run_generate(args) -> int:
         from .cache import BLOCK_TOKENS          # requests hold the cache in whole blocks
         cache_tokens = sum(-(-(len(p) + max(1, args.max_tokens)) // BLOCK_TOKENS) * BLOCK_TOKENS for p in prompts) + BLOCK_TOKENS
     if args.model:
-        runtime = Runtime.load(args.model, dtype=args.dtype, max_tokens=cache_tokens, int8_weights=args.int8_weights)
+        runtime = Runtime.load(args.model, dtype=args.dtype, max_tokens=cache_tokens)
     else:
         with open(args.random) as handle:
             config = parse_config(json.load(handle))
-        runtime = Runtime.random(config, seed=args.seed or 0, dtype=args.dtype, max_tokens=cache_tokens, int8_weights=args.int8_weights)
+        runtime = Runtime.random(config, seed=args.seed or 0, dtype=args.dtype, max_tokens=cache_tokens)
     requests = [GenerateRequest(p, max_tokens=args.max_tokens, temperature=args.temperature, top_k=args.top_k,
                                 top_p=args.top_p, repetition_penalty=args.repetition_penalty, seed=args.seed,
                                 stop_ids=stops) for p in prompts]

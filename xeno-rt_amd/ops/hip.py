@@ -586,18 +586,11 @@ class HipOps:
         """out (+)= a w^T. `a` may be a Prescaled. then_norm = (gain, eps) of an RMSNorm that follows an
         accumulating product: if this product can, it returns the normed rows of the updated `out` for the
         product after the norm (a Prescaled, whose division that product does; with many rows the normed
-        rows themselves); None means that the caller runs the norm. w may be an Int8Matrix: `linear_int8`, of rows that are
-        brought to 8 bits first if they are not Int8Rows already."""
-        if isinstance(w, Int8Matrix):
-            self.linear_int8(self._as_int8(a, w), w, out, accumulate=accumulate)
-            return None
+        rows themselves); None means that the caller runs the norm."""
         return self._linear(a, w, out, 1 if accumulate else 0, w.shape[0], then_norm)
 
     def linear_glu(self, a, w_gate_up, out, activation: str = "silu"):
-        """out = act(a w_gate^T) * (a w_up^T) with w_gate_up = [gate rows | up rows], which may be a gated Int8Matrix as in `linear`."""
-        if isinstance(w_gate_up, Int8Matrix):
-            self.linear_glu_int8(self._as_int8(a, w_gate_up), w_gate_up, out, activation=activation)
-            return
+        """out = act(a w_gate^T) * (a w_up^T) with w_gate_up = [gate rows | up rows]."""
         if w_gate_up.shape[0] % 2 != 0:
             raise KernelError("linear_glu: the weight needs gate rows followed by as many up rows")
         if activation not in ACTIVATIONS:
@@ -629,16 +622,6 @@ class HipOps:
             self._require(tensor, what, dtype, shape)
             raise KernelError(f"{what}: on {tensor.device}, expected cuda:{index}")
         return tensor.data_ptr()
-
-    def _as_int8(self, a, w: "Int8Matrix") -> Int8Rows:
-        """What a product with w reads: a, in 8 bits."""
-        if isinstance(a, Int8Rows):
-            return a
-        if not isinstance(a, torch.Tensor) or a.dim() != 2:
-            raise KernelError("linear: a product with 8-bit weights reads rows [rows, k] or Int8Rows")
-        rows = self.int8_rows(a.shape[0], a.shape[1], a.device)
-        self.quantize_int8(a, rows)
-        return rows
 
     def int8_rows(self, rows: int, k: int, device) -> Int8Rows:
         """Room for `rows` rows of k columns in 8-bit integers; what it holds is not defined."""
@@ -770,12 +753,7 @@ class HipOps:
 
     def linear_qkv(self, a, w, qkv, n_heads, n_kv_heads, head_dim, positions, slots, q_norm=None, k_norm=None,
                    norm_eps=0.0, rope_theta=None, rope_dim=0, rope_scale=1.0, kv=None, longest_run=0):
-        """qkv = a w^T, then qkv_prepare of it: one kernel where a step is short enough. `a` may be a Prescaled; w an Int8Matrix as in `linear`."""
-        if isinstance(w, Int8Matrix):
-            self.linear(a, w, qkv)
-            self.qkv_prepare(qkv, n_heads, n_kv_heads, head_dim, positions, slots, q_norm=q_norm, k_norm=k_norm, norm_eps=norm_eps,
-                             rope_theta=rope_theta, rope_dim=rope_dim, rope_scale=rope_scale, kv=kv, longest_run=longest_run)
-            return
+        """qkv = a w^T, then qkv_prepare of it: one kernel where a step is short enough. `a` may be a Prescaled."""
         scaled = a if isinstance(a, Prescaled) else None
         if scaled is not None:
             a = scaled.values

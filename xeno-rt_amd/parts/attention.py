@@ -234,10 +234,9 @@ class Attention(Mixer):
         rotation = None if self.position is None else self.position.rotation()
         whole = rotation is not None and rotation.rope_dim == self.head_dim
         self.w_qkv = runtime.weight([tensors[p + n[name]] for name in "qkv"],
-                                    "rotary", int8=True, head_dim=self.head_dim,
+                                    "rotary", head_dim=self.head_dim,
                                     rotated_heads=self.n_heads + self.n_kv_heads if whole else 0)
-        self.w_o = runtime.weight(tensors[p + n["o"]], int8=True)
-        self.reads_int8 = runtime.int8_weights
+        self.w_o = runtime.weight(tensors[p + n["o"]])
         if self.qk_norm:
             self.q_norm = runtime.vector(tensors[p + n["q_norm"]])
             self.k_norm = runtime.vector(tensors[p + n["k_norm"]])
@@ -321,7 +320,7 @@ class Attention(Mixer):
     @property
     def one_call(self) -> bool:
         """Whether `describe` says all there is to say of this layer: plain causal attention, positions by rotation or not at all."""
-        return type(self) is Attention and not self.general and not self.reads_int8 and self.window is None and (self.position is None or self.position.rotation() is not None) and (
+        return type(self) is Attention and not self.general and self.window is None and (self.position is None or self.position.rotation() is not None) and (
             self.position is None or self.position.score_slopes() is None)
 
     # Tokens whose results nobody wants need go no further than the cache behind the model's last attention: the others alone go on from there,

@@ -142,7 +142,7 @@ class StepArena:
 class Runtime:
     """What a part needs to run: the kernels, the compute dtype and the device."""
 
-    def __init__(self, ops, dtype: torch.dtype, device, pack_weights="auto", int8_weights: bool = False):
+    def __init__(self, ops, dtype: torch.dtype, device, pack_weights="auto"):
         if dtype not in (torch.bfloat16, torch.float32):
             raise ValueError(f"compute dtype must be bfloat16 or float32, found {dtype}")
         if pack_weights not in ("auto", "always", False):
@@ -151,7 +151,6 @@ class Runtime:
         self.dtype = dtype
         self.device = torch.device(device)
         self.pack_weights = pack_weights        # "auto": where the kernels say it pays; "always": wherever it can be done
-        self.int8_weights = bool(int8_weights)  # matrices of parts that say `int8` to `weight` are kept in 8-bit integers
         self.arena = StepArena(self.device)     # what `empty` cuts a step's tensors from, while a step is under way
 
     def matrix(self, tensor: torch.Tensor) -> torch.Tensor:
@@ -177,18 +176,15 @@ class Runtime:
             at += tensor.shape[0]
         return out
 
-    def weight(self, tensors, kind: str = "tiles", needed: bool = False, int8: bool = False, **details):
+    def weight(self, tensors, kind: str = "tiles", needed: bool = False, **details):
         """What `ops.linear` (or `linear_glu`, `linear_qkv`, `embed`) takes as its w: the matrix (or the matrices
         of equal width, one below the other) in the compute dtype on the device, and, where the kernels have a
         faster layout for matrices of its sizes, in that layout. kind and details name what the product's
         epilogue combines: "tiles" nothing, "gated" gate rows and up rows (gated_n of each), "rotary" the
         pairs of a rotation over whole heads (head_dim, rotated_heads). needed: some kernel reads the faster layout as such
         (not only faster), so it is made wherever it can be, also at sizes where it would not pay by itself. Only products
-        read the result. int8: nothing but `ops.linear`, `linear_glu` and `linear_qkv` reads it, so that it may be kept in 8-bit integers with
-        a scale for each row (`ops.pack_int8`), as it is where the runtime was told so."""
+        read the result."""
         matrix = self.stacked(tensors) if isinstance(tensors, (list, tuple)) else self.matrix(tensors)
-        if int8 and self.int8_weights:
-            return self.ops.pack_int8(matrix, gated=kind == "gated")
         pack = getattr(self.ops, "pack", None)
         if (pack is None or not self.pack_weights or self.dtype != torch.bfloat16 or matrix.device.type != "cuda"
                 or matrix.shape[1] % 32 != 0 or (matrix.shape[0] + 15) * matrix.shape[1] >= 2 ** 31):
@@ -253,9 +249,6 @@ class Part:
     # Parts that look at the batch on the host (loops over sequences, Python arithmetic on
     # lengths) leave it False; a model with such a part runs every step directly.
     capturable = False
-    # True if the part reads its rows in 8 bits (its first product's weight is kept so): a norm before it
-    # that can make them (`forward_int8`) then does. It reads plain rows as well.
-    reads_int8 = False
 
     def weight_specs(self) -> Dict[str, WeightSpec]:
         """Full checkpoint name -> WeightSpec of every tensor this part binds."""

@@ -61,8 +61,7 @@ class PreNormBlock(Block):
         return plain and bool(getattr(self.mixer, "passes_norms", False))
 
     def first_norm(self):
-        # (a mixer that reads rows in 8 bits takes no norm that the product before it has begun)
-        return None if getattr(self.mixer, "reads_int8", False) else self.mixer_norm
+        return self.mixer_norm
 
     @staticmethod
     def _read(x, norm, transform, batch, cache):
@@ -74,11 +73,6 @@ class PreNormBlock(Block):
             return transform.forward_normed(x, norm, batch, cache)
         return transform.forward(norm.forward(x), batch, cache)
 
-    @staticmethod
-    def _normed(x, norm, reader):
-        """The normed rows as the part after the norm reads them."""
-        return norm.forward_int8(x) if getattr(reader, "reads_int8", False) and hasattr(norm, "forward_int8") else norm.forward(x)
-
     def forward(self, x, batch, cache, h=None, then=None):
         if not self.passes_norms:
             self.mixer.forward(self._read(x, self.mixer_norm, self.mixer_input, batch, cache), batch, cache, x)
@@ -86,14 +80,14 @@ class PreNormBlock(Block):
                 self.feed_forward.forward(self._read(x, self.feed_forward_norm, self.feed_forward_input, batch, cache), batch, x)
             return None
         if h is None:
-            h = self._normed(x, self.mixer_norm, self.mixer)
+            h = self.mixer_norm.forward(x)
         # a norm is left to the products around it only if the part after it reads nothing but products of it
-        if self.passes_norms and getattr(self.feed_forward, "passes_norms", False) and not getattr(self.feed_forward, "reads_int8", False):
+        if self.passes_norms and getattr(self.feed_forward, "passes_norms", False):
             h = self.mixer.forward(h, batch, cache, x, then=self.feed_forward_norm)
         else:
             h = self.mixer.forward(h, batch, cache, x)
         if h is None:
-            h = self._normed(x, self.feed_forward_norm, self.feed_forward)
+            h = self.feed_forward_norm.forward(x)
         if then is not None and getattr(self.feed_forward, "passes_norms", False):
             return self.feed_forward.forward(h, batch, x, then=then)
         self.feed_forward.forward(h, batch, x)

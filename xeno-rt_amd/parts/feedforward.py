@@ -43,14 +43,13 @@ class GatedMLP(FeedForward):
 
     def bind(self, tensors, runtime: Runtime) -> None:
         super().bind(tensors, runtime)
-        self.w_gate_up = runtime.weight([tensors[self.gate_name], tensors[self.up_name]], "gated", int8=True, gated_n=self.intermediate)
-        self.w_down = runtime.weight(tensors[self.down_name], int8=True)
-        self.reads_int8 = runtime.int8_weights
+        self.w_gate_up = runtime.weight([tensors[self.gate_name], tensors[self.up_name]], "gated", gated_n=self.intermediate)
+        self.w_down = runtime.weight(tensors[self.down_name])
 
     @property
     def one_call(self) -> bool:
         """Whether `describe` says all there is to say of this feed-forward."""
-        return type(self) is GatedMLP and self.activation == "silu" and not self.reads_int8
+        return type(self) is GatedMLP and self.activation == "silu"
 
     def describe(self, record, hidden: int, device: int) -> None:
         """This feed-forward in the record that `ops.dense_blocks` reads, for a stream of width `hidden`."""

@@ -44,13 +44,6 @@ class RMSNorm(Norm):
         self.runtime.ops.rmsnorm(x, self.weight, self.eps, out, rows=rows)
         return out
 
-    def forward_int8(self, x: torch.Tensor):
-        """The same rows in 8-bit integers (`ops.rmsnorm_int8`), for products with weights kept so."""
-        ops = self.runtime.ops
-        out = ops.int8_rows(x.shape[0], self.dim, x.device)
-        ops.rmsnorm_int8(x, self.weight, self.eps, out)
-        return out
-
     def add_to(self, residual: torch.Tensor, y: torch.Tensor, scale: float = 1.0, copy: Optional[torch.Tensor] = None) -> None:
         """residual += scale * norm(y); y float32 like the residual. copy, if given, takes the updated rows in its own element type."""
         self.runtime.ops.add_normed(residual, [(y, self.weight)], self.eps, scale, **({} if copy is None else {"copy": copy}))
