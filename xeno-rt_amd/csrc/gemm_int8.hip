@@ -526,16 +526,16 @@ struct Plan {
 
 Plan plan_of(long M, long groups, long stride) {
     const long units = stride / XRT_INT8_STEP;
-    // The kernel of few rows: up to 64, and more where its tiles of 64 x 64 find a compute unit each and no workgroup goes through more than 7168 columns (a
-    // tile reads as much of a as of w). It takes a half to nine tenths of the time of the larger tiles there (217 rows, k = 384, 1312 channels 6.9 -> 4.5 us;
-    // 447, 1536, 1440 14.0 -> 7.6; 456, 7168, 912 pairs 23.7 -> 21.0; 239, 7552, 1496 pairs 20.9 -> 22.7).
+    // The kernel of few rows: up to 64, and more where its tiles of 64 x 64 find a compute unit each and no workgroup goes through more than 7168 columns (5120 of a
+    // k in parts; a tile reads as much of a as of w). It takes a half to nine tenths of the time of the larger tiles there (217 rows, k = 384, 1312 channels 6.9 -> 4.5 us;
+    // 447, 1536, 1440 14.0 -> 7.6; 456, 7168, 912 pairs 23.7 -> 21.0; 239, 7552, 1496 pairs 20.9 -> 22.7; 100, 14336, 4096 channels 22.4 in eight parts, 26.1 in two).
     {
         // (two blocks of rows, 1792 groups of w: 27.7 us with two groups a workgroup, 24.5 with four; 384 groups: 9.5 and 11.1)
         Plan plan{0, 0, M <= 16 ? 1 : M <= 32 ? 2 : 4, M <= 16 ? 1 : M <= 32 && groups < 4 * XRT_COMPUTE_UNITS ? 2 : 4, 1};
         const long workgroups = (M + plan.blocks * 16 - 1) / (plan.blocks * 16) * ((groups + plan.groups - 1) / plan.groups);
         const long most = plan.blocks == 1 ? XRT_COMPUTE_UNITS / 2 : XRT_COMPUTE_UNITS;
         while (plan.parts < 8 && workgroups * plan.parts * 2 <= most && units / (plan.parts * 2) >= 4) plan.parts *= 2;
-        if (M <= 64 || (workgroups <= XRT_COMPUTE_UNITS && units <= plan.parts * 56)) return plan;
+        if (M <= 64 || (workgroups <= XRT_COMPUTE_UNITS && units <= (plan.parts == 1 ? 56 : 40 * plan.parts))) return plan;
     }
     // What a tile height costs, fitted to products of 4096 rows, k = 4096 and 14336 (us): a step along k (256 rows: 1.31, 128: 0.80), and the first loads and the
     // epilogue. A partly filled round takes half of a full one and its share of the rest: power bounds the chip, and the compute units at work run faster.
@@ -627,6 +627,13 @@ extern "C" long xrt_linear_int8_workspace(int M, int N, int K, int mode) {
     if (M <= 0 || N <= 0 || K <= 0 || K > XRT_INT8_MOST_K) return 0;
     const long groups = int8_groups(N, mode_of(mode) == MODE_GATED);
     return sums_bytes(plan_of(M, groups, int8_stride(K)), M, groups);
+}
+
+extern "C" int xrt_linear_int8_plan(int M, int N, int K, int mode, int* plan) {
+    XRT_REQUIRE(plan && M > 0 && N > 0 && K > 0 && K <= XRT_INT8_MOST_K, "linear_int8: bad sizes M=%d N=%d K=%d", M, N, K);
+    const Plan chosen = plan_of(M, int8_groups(N, mode_of(mode) == MODE_GATED), int8_stride(K));
+    plan[0] = chosen.tile, plan[1] = chosen.width, plan[2] = chosen.blocks, plan[3] = chosen.groups, plan[4] = chosen.parts;
+    return 0;
 }
 
 extern "C" int xrt_linear_int8(const void* a, const float* a_scales, const void* w, const float* w_scales, void* out, int out_dtype, int M, int N, int K,

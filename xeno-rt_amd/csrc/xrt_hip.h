@@ -130,6 +130,9 @@ int xrt_pack_int8(const void* values, const float* scales, void* packed, float* 
 int xrt_linear_int8(const void* a, const float* a_scales, const void* w, const float* w_scales, void* out, int out_dtype, int M, int N, int K,
                     int mode, void* workspace, long workspace_bytes, void* stream);
 long xrt_linear_int8_workspace(int M, int N, int K, int mode);
+// What such a product takes, for tests: plan[0], plan[1] the rows of a and the packed rows of w of a tile in LDS (0, 0: it is streamed through registers, plan[2]
+// blocks of 16 rows of a and plan[3] groups of 16 packed rows of w a workgroup), plan[4] the parts that k is cut into.
+int xrt_linear_int8_plan(int M, int N, int K, int mode, int* plan);
 
 // An RMSNorm between two products, x += a w^T; y = rmsnorm(x) * gain; z = y v^T, without a kernel of
 // its own. The first product (mode 1) also writes scaled_out[m, n] = bfloat16(x[m, n] * gain[n]) and
