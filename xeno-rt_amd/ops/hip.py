@@ -633,33 +633,39 @@ class HipOps:
     def quantize_int8(self, x, out: Int8Rows):
         """out = the rows of x (float32 or bfloat16, some columns of a wider matrix will do) in 8-bit integers: scales[m] = max |x[m]| / 127, values =
         x / scale rounded to the nearest integer, halves to even. A row of zeros has scale 0; one that holds an infinity or a NaN scale NaN and zeros."""
-        stride, index = self._rows(x, "quantize_int8 x"), x.get_device()
-        self._is_int8(out, "quantize_int8 out", x.shape, index)
+        if isinstance(out, Int8Rows) and isinstance(x, torch.Tensor) and x.shape == out.shape and x.is_contiguous() and x.get_device() == out.index:
+            stride, index = out.shape[1], out.index
+        else:
+            stride, index = self._rows(x, "quantize_int8 x"), x.get_device()
+            self._is_int8(out, "quantize_int8 out", x.shape, index)
         rows, k = out.shape
-        self._check(self.lib.xrt_quantize_int8(x.data_ptr(), _code(x), stride, out._values.data_ptr(), out._scales.data_ptr(), rows, k, self._int8_stream(index)))
+        status = self.lib.xrt_quantize_int8(x.data_ptr(), _code(x), stride, out._values.data_ptr(), out._scales.data_ptr(), rows, k, self._int8_stream(index))
+        if status != 0:
+            self._check(status)
 
     def rmsnorm_int8(self, x, weight, eps, out: Int8Rows, delta=None, rows=None):
         """x += delta in place, if given (float32 or bfloat16, shaped like x), then out = the rows x / sqrt(mean(x^2) + eps) * weight as `quantize_int8`
         would make them of float32. x is float32. rows: the rows of x that are wanted, as in `rmsnorm` (not together with delta); one that x does not
         have gives zeros with scale NaN."""
-        self._require(x, "rmsnorm_int8 x", torch.float32)
-        if x.dim() != 2:
-            raise KernelError("rmsnorm_int8 x: expected [rows, hidden]")
-        (x_rows, hidden), index = x.shape, x.get_device()
-        at_weight = self._is_tensor(weight, "rmsnorm_int8 weight", None, (hidden,), index)
-        count, at_rows, at_delta, delta_code = x_rows, None, None, 0
+        if not isinstance(out, Int8Rows):
+            raise KernelError("rmsnorm_int8 out: expected Int8Rows")
+        (count, hidden), index = out.shape, out.index
+        x_rows, at_rows, at_delta, delta_code = count, None, None, 0
         if rows is not None:
             if delta is not None:
                 raise KernelError("rmsnorm_int8: chosen rows of x cannot be added to (one might be chosen twice)")
-            if not isinstance(rows, torch.Tensor) or rows.dim() != 1:
-                raise KernelError("rmsnorm_int8 rows: expected a list of rows on the GPU")
-            count = rows.shape[0]
             at_rows = self._is_tensor(rows, "rmsnorm_int8 rows", torch.int32, (count,), index)
-        elif delta is not None:
-            at_delta, delta_code = self._is_tensor(delta, "rmsnorm_int8 delta", None, x.shape, index), _code(delta)
-        self._is_int8(out, "rmsnorm_int8 out", (count, hidden), index)
-        self._check(self.lib.xrt_rmsnorm_int8(x.data_ptr(), at_delta, delta_code, at_weight, _code(weight), eps, out._values.data_ptr(), out._scales.data_ptr(),
-                                              at_rows, count, x_rows, hidden, self._int8_stream(index)))
+            if not isinstance(x, torch.Tensor) or x.dim() != 2:
+                raise KernelError("rmsnorm_int8 x: expected [rows, hidden]")
+            x_rows = x.shape[0]
+        at_x = self._is_tensor(x, "rmsnorm_int8 x", torch.float32, (x_rows, hidden), index)
+        at_weight = self._is_tensor(weight, "rmsnorm_int8 weight", None, (hidden,), index)
+        if delta is not None:
+            at_delta, delta_code = self._is_tensor(delta, "rmsnorm_int8 delta", None, out.shape, index), _code(delta)
+        status = self.lib.xrt_rmsnorm_int8(at_x, at_delta, delta_code, at_weight, _code(weight), eps, out._values.data_ptr(), out._scales.data_ptr(), at_rows, count,
+                                           x_rows, hidden, self._int8_stream(index))
+        if status != 0:
+            self._check(status)
 
     def dequantize_int8(self, rows: Int8Rows, out):
         """out[m, j] = values[m, j] * scales[m] (float32 or bfloat16)."""
@@ -667,7 +673,9 @@ class HipOps:
             raise KernelError("dequantize_int8 rows: expected Int8Rows")
         (count, k), index = rows.shape, rows.index
         at_out = self._is_tensor(out, "dequantize_int8 out", None, rows.shape, index)
-        self._check(self.lib.xrt_dequantize_int8(rows._values.data_ptr(), rows._scales.data_ptr(), at_out, _code(out), count, k, self._int8_stream(index)))
+        status = self.lib.xrt_dequantize_int8(rows._values.data_ptr(), rows._scales.data_ptr(), at_out, _code(out), count, k, self._int8_stream(index))
+        if status != 0:
+            self._check(status)
 
     def pack_int8(self, w, gated: bool = False) -> Int8Matrix:
         """The weight matrix w [rows, k] for `linear_int8`, or gated ([gate rows | up rows]) for `linear_glu_int8`: Int8Rows, or a float matrix, whose
@@ -691,18 +699,19 @@ class HipOps:
 
     def _linear_int8(self, a, w, out, mode, n):
         k, index = w.shape[1], w.index
-        if not isinstance(a, Int8Rows):
-            raise KernelError("8-bit product: a must be Int8Rows")
+        if not isinstance(a, Int8Rows) or a.shape[1] != k or a.index != index:
+            self._is_int8(a, "8-bit product a", (a.shape[0] if isinstance(a, Int8Rows) else 0, k), index)
         m = a.shape[0]
-        self._is_int8(a, "8-bit product a", (m, k), index)
         at_out, code = self._is_tensor(out, "8-bit product out", None, (m, n), index), _code(out)
         if mode == 1 and code != 0:
             raise KernelError(f"linear_int8 out: added to in {out.dtype}, expected float32")
         stream = self._int8_stream(index)
         need = self.lib.xrt_linear_int8_workspace(m, n, k, mode)
         workspace = self._empty(need // 4, torch.int32, out.device) if need > 0 else None
-        self._check(self.lib.xrt_linear_int8(a._values.data_ptr(), a._scales.data_ptr(), w.data.data_ptr(), w.scales.data_ptr(), at_out, code, m, n, k, mode,
-                                             None if workspace is None else workspace.data_ptr(), need, stream))
+        status = self.lib.xrt_linear_int8(a._values.data_ptr(), a._scales.data_ptr(), w.data.data_ptr(), w.scales.data_ptr(), at_out, code, m, n, k, mode,
+                                          None if workspace is None else workspace.data_ptr(), need, stream)
+        if status != 0:
+            self._check(status)
 
     def linear_int8(self, a: Int8Rows, w: Int8Matrix, out, accumulate=False):
         """out[m, n] (+)= (sum over j of a[m, j] w[n, j], exact) * a.scales[m] * w.scales[n], in float32; out is float32 or bfloat16, float32 if it is
