@@ -193,7 +193,9 @@ def near(out, want, base=None):
 # one row and one column, sizes around the tiles of 16, 64, 128 and 256 and around steps of 64 and 128 along k, long and short k, odd sizes of everything
 SIZES = [(1, 1, 1), (1, 5, 64), (2, 16, 65), (3, 17, 127), (1, 4096, 4096), (5, 300, 129), (16, 1000, 512), (17, 48, 1000), (31, 130, 4100), (33, 512, 14336), (48, 4096, 256),
          (64, 257, 2048), (65, 640, 1024), (100, 1001, 777), (128, 128, 128), (129, 255, 300), (200, 3000, 512), (255, 256, 64), (256, 256, 640), (257, 513, 1280), (333, 1280, 5120),
-         (512, 6144, 1024), (777, 1001, 2049), (1030, 2050, 384), (2048, 512, 2048), (9, 40000, 128), (300, 24, 9000)]
+         (512, 6144, 1024), (777, 1001, 2049), (1030, 2050, 384), (2048, 512, 2048), (9, 40000, 128), (300, 24, 9000),
+         # 17 to 32 rows of many channels; the larger tiles, with rows and channels that do not fill the last one, one step along k and an odd number of them
+         (20, 16400, 256), (300, 16000, 640), (500, 9000, 500), (1200, 8200, 256), (190, 40000, 100), (70, 5000, 8000), (2049, 7000, 384), (3333, 4111, 120), (800, 12345, 128), (1030, 20000, 128), (10, 100, 9000), (25, 3000, 200)]
 
 
 @pytest.mark.parametrize("m,n,k", SIZES)
@@ -226,8 +228,8 @@ def test_gated_products_of_8_bit_rows(ops, m, n, k):
         assert bool((out[0] == 77.0).all()) and bool((out[m + 1] == 77.0).all())
 
 
-def test_a_row_has_the_same_bits_alone_and_among_others(ops):
-    n, k = 700, 3000
+@pytest.mark.parametrize("n,k", [(700, 3000), (12000, 300)])
+def test_a_row_has_the_same_bits_alone_and_among_others(ops, n, k):
     a, w = whole_numbers(600, k, seed=1), ops.pack_int8(whole_numbers(n, k, seed=2))
     gated = ops.pack_int8(whole_numbers(n, k, seed=3), gated=True)
     from xeno_rt_amd.ops.hip import Int8Rows
@@ -281,11 +283,45 @@ def test_weights_packed_from_floats(ops):
             assert torch.equal(one.data, two.data) and torch.equal(one.scales, two.scales) and one.shape == (70, 333)
 
 
+def test_what_lies_behind_the_columns_does_not_count(ops):
+    for m in (3, 40, 300):
+        for k in (1, 100, 130, 500):
+            a, w = whole_numbers(m, k, seed=1), whole_numbers(40, k, seed=2)
+            want, gated = torch.empty(m, 40, device=DEV), torch.empty(m, 20, device=DEV)
+            ops.linear_int8(a, ops.pack_int8(w), want)
+            ops.linear_glu_int8(a, ops.pack_int8(w, gated=True), gated)
+            a.values[:, k:], w.values[:, k:] = 77, -99
+            got, got_gated = torch.empty_like(want), torch.empty_like(gated)
+            ops.linear_int8(a, ops.pack_int8(w), got)
+            ops.linear_glu_int8(a, ops.pack_int8(w, gated=True), got_gated)
+            assert torch.equal(got, want) and torch.equal(got_gated, gated)
+
+
+def test_tensors_of_another_device_than_the_current_one_are_refused(ops, monkeypatch):
+    from xeno_rt_amd.ops import hip
+    q, w, x = ops.int8_rows(4, 100, DEV), ops.pack_int8(rand(20, 100)), rand(4, 100)
+    monkeypatch.setattr(hip, "_current_device", lambda: 1)
+    for call in (lambda: ops.quantize_int8(x, q), lambda: ops.rmsnorm_int8(x, rand(100), EPS, q), lambda: ops.dequantize_int8(q, x), lambda: ops.pack_int8(x),
+                 lambda: ops.linear_int8(q, w, rand(4, 20))):
+        with pytest.raises(hip.KernelError, match="current device"):
+            call()
+
+
+def test_a_norm_whose_addend_is_the_stream_itself(ops):
+    for k in (300, 40007):
+        x = rand(3, k, seed=4)
+        want, out, plain = x + x, ops.int8_rows(3, k, DEV), ops.int8_rows(3, k, DEV)
+        ops.rmsnorm_int8(x, torch.ones(k, device=DEV), EPS, out, delta=x)
+        ops.rmsnorm_int8(want.clone(), torch.ones(k, device=DEV), EPS, plain)
+        assert torch.equal(x, want) and torch.equal(out.values, plain.values) and torch.equal(out.scales, plain.scales)
+
+
 def test_no_rows(ops):
     w, gated = ops.pack_int8(rand(20, 100)), ops.pack_int8(rand(20, 100), gated=True)
     a = ops.int8_rows(0, 100, DEV)
     ops.quantize_int8(rand(0, 100), a)
     ops.rmsnorm_int8(rand(0, 100), rand(100), EPS, a, delta=rand(0, 100))
+    ops.rmsnorm_int8(rand(5, 100), rand(100), EPS, a, rows=torch.empty(0, dtype=torch.int32, device=DEV))
     ops.dequantize_int8(a, rand(0, 100))
     ops.linear_int8(a, w, rand(0, 20))
     ops.linear_glu_int8(a, gated, rand(0, 10))
@@ -380,7 +416,7 @@ def test_two_captured_graphs_and_two_streams_at_once(ops):
 # ---- refusals ---------------------------------------------------------------------------------------------------------------------------------------------------
 
 def test_refusals(ops):
-    from xeno_rt_amd.ops.hip import INT8_MOST_K, Int8Rows, KernelError
+    from xeno_rt_amd.ops.hip import INT8_MOST_K, Int8Matrix, Int8Rows, KernelError
     q, w, gated = ops.int8_rows(4, 100, DEV), ops.pack_int8(rand(20, 100)), ops.pack_int8(rand(20, 100), gated=True)
     x, gain = rand(4, 100), rand(100)
     refused = [
@@ -401,6 +437,9 @@ def test_refusals(ops):
         lambda: ops.linear_int8(q, w, rand(4, 40)[:, ::2]), lambda: Int8Rows(q.values[:, :100], q.scales, 100), lambda: Int8Rows(q.values.cpu(), q.scales, 100), lambda: Int8Rows(q.values[0], q.scales, 100), lambda: Int8Rows(q.values, q.scales, 129),
         lambda: Int8Rows(q.values.view(-1)[:-1].clone(), q.scales, 100), lambda: Int8Rows(torch.empty(4 * 128 + 8, dtype=torch.int8, device=DEV)[8:].view(4, 128), q.scales, 100),
         lambda: Int8Rows(q.values, q.scales[:3], 100), lambda: Int8Rows(q.values, q.scales.cpu(), 100), lambda: Int8Rows(q.values, q.scales, 0),
+        lambda: Int8Matrix(w.data, w.scales, 20, 129, False), lambda: Int8Matrix(w.data, w.scales, 33, 100, False), lambda: Int8Matrix(w.data, w.scales[:8], 20, 100, False),
+        lambda: Int8Matrix(w.data.view(torch.uint8), w.scales, 20, 100, False), lambda: Int8Matrix(gated.data, gated.scales, 21, 100, True),
+        lambda: ops.rmsnorm_int8(x, gain, EPS, x), lambda: ops.linear_int8(Int8Rows(q.values, q.scales, 101), w, rand(4, 20)),
         lambda: ops.linear_glu_int8(q, w, rand(4, 10)), lambda: ops.linear_glu_int8(q, gated, rand(4, 20)), lambda: ops.linear_glu_int8(q, gated, rand(4, 10), activation="relu"),
     ]
     for index, call in enumerate(refused):

@@ -550,9 +550,10 @@ Plan plan_of(long M, long groups, long stride) {
         if (plan.tile == 0 || cost < best) plan.tile = tile, best = cost;
     }
     long tiles = (M + plan.tile - 1) / plan.tile * tiles_n;
-    // Tiles half as wide where the others fill up to half of the chip: a compute unit has a limit of its own on what it has asked for of w.
+    // Tiles half as wide where the others fill up to half of the chip, and k in parts as far as every compute unit gets one at most: a compute unit pulls no more
+    // than some 29 GB/s of w, however much is asked for ahead (100 rows, k = 4096, 14336 pairs 34.5 us in 112 tiles, 28.7 in 224; three steps in LDS instead of two changed nothing).
     if (plan.tile == 128 && tiles * 2 <= XRT_COMPUTE_UNITS) plan.width = 128, tiles = (M + 127) / 128 * ((groups + 7) / 8);
-    while (plan.parts < 16 && tiles * plan.parts * 2 <= XRT_COMPUTE_UNITS && units / (plan.parts * 2) >= 3) plan.parts *= 2;
+    while (plan.width == 128 && plan.parts < 16 && tiles * plan.parts * 2 <= XRT_COMPUTE_UNITS && units / (plan.parts * 2) >= 3) plan.parts *= 2;
     const long steps = (units + plan.parts - 1) / plan.parts;
     plan.parts = (int)((units + steps - 1) / steps);           // (none is empty)
     return plan;
@@ -562,13 +563,14 @@ long sums_bytes(const Plan& plan, long M, long groups) { return plan.parts == 1 
 
 struct Operands { const signed char* a; const signed char* w; int4v* sums; int stride, groups; hipStream_t stream; };
 
-template <int MT, int G, int MODE, typename TO, bool ONCE = true>
+template <int MT, int G, int MODE, typename TO, bool ONCE = true, bool SPLITS = true>
 int launch_few(const Operands& o, const Plan& plan, const Result<TO>& to) {
     const int tiles_m = (to.M + MT * 16 - 1) / (MT * 16), tiles_n = (o.groups + G - 1) / G;
     const long ids = part_ids((long)tiles_m * tiles_n, plan.parts, true);        // a whole number of rounds over the XCDs
     XRT_REQUIRE(ids < (1L << 31), "linear_int8: %ld tiles", ids);
     if (plan.parts == 1) gemm_int8_few_kernel<MT, G, MODE, TO, false, ONCE><<<(unsigned)ids, WAVES * XRT_WAVE, 0, o.stream>>>(o.a, o.w, nullptr, to.M, o.stride, o.groups, tiles_m, tiles_n, 1, to);
-    else gemm_int8_few_kernel<MT, G, MODE_STORE, float, true, ONCE><<<(unsigned)ids, WAVES * XRT_WAVE, 0, o.stream>>>(o.a, o.w, o.sums, to.M, o.stride, o.groups, tiles_m, tiles_n, plan.parts, Result<float>{});
+    else if constexpr (SPLITS) gemm_int8_few_kernel<MT, G, MODE_STORE, float, true, ONCE><<<(unsigned)ids, WAVES * XRT_WAVE, 0, o.stream>>>(o.a, o.w, o.sums, to.M, o.stride, o.groups, tiles_m, tiles_n, plan.parts, Result<float>{});
+    XRT_REQUIRE(SPLITS || plan.parts == 1, "linear_int8: a product that is not cut, in %d parts", plan.parts);
     return 0;
 }
 
@@ -598,16 +600,14 @@ int launch(const Operands& o, const Plan& plan, const Result<TO>& to) {
     if (plan.tile == 0) {
         if (plan.blocks == 1) failed = launch_few<1, 1, MODE, TO>(o, plan, to);
         else if (plan.blocks == 2 && plan.groups == 2) failed = launch_few<2, 2, MODE, TO>(o, plan, to);
-        else if (plan.blocks == 2) failed = launch_few<2, 4, MODE, TO>(o, plan, to);
+        else if (plan.blocks == 2) failed = launch_few<2, 4, MODE, TO, true, false>(o, plan, to);      // (1024 groups and more: never cut)
         else if (to.M <= 64) failed = launch_few<4, 4, MODE, TO>(o, plan, to);
         else failed = launch_few<4, 4, MODE, TO, false>(o, plan, to);
     } else if (plan.parts > 1) {
         Result<float> sizes{};
         sizes.M = to.M, sizes.N = to.N;
-        if (plan.tile == 256) failed = launch_large<256, 256, MODE_STORE, float, true>(o, plan, sizes);
-        else if (plan.tile == 192) failed = launch_large<192, 256, MODE_STORE, float, true>(o, plan, sizes);
-        else if (plan.width == 256) failed = launch_large<128, 256, MODE_STORE, float, true>(o, plan, sizes);
-        else failed = launch_large<128, 128, MODE_STORE, float, true>(o, plan, sizes);
+        XRT_REQUIRE(plan.tile == 128 && plan.width == 128, "linear_int8: tiles of %d x %d in parts", plan.tile, plan.width);
+        failed = launch_large<128, 128, MODE_STORE, float, true>(o, plan, sizes);       // (products that are cut have few tiles: the small ones)
     } else if (plan.tile == 256) failed = launch_large<256, 256, MODE, TO, false>(o, plan, to);
     else if (plan.tile == 192) failed = launch_large<192, 256, MODE, TO, false>(o, plan, to);
     else if (plan.width == 256) failed = launch_large<128, 256, MODE, TO, false>(o, plan, to);

@@ -1,7 +1,7 @@
 // Rows and weight matrices in 8-bit integers with scales.
 //
-// Rows: values[m][j] (signed bytes, a row every int8_stride(k) bytes, zeros behind the k columns) and scales[m] (float32); row m stands for
-// values[m][j] * scales[m]. The zeros let every product run in whole steps of 128 along k, whatever k is.
+// Rows: values[m][j] (signed bytes, a row every int8_stride(k) bytes) and scales[m] (float32); row m stands for values[m][j] * scales[m]. Behind the k
+// columns the operators write zeros, and packed weights have zeros there in any case, so that every product runs in whole steps of 128 along k.
 //
 // A weight matrix w[rows][k] is kept in tiles of 16 rows x 64 columns, 1 KB each, the tiles of a group of 16 rows one after another along k, groups one
 // after another. Inside a tile the 16-byte pieces (16 columns of one row) lie in the order in which the lanes of a wavefront hold the A operand of

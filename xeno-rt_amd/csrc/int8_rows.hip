@@ -203,7 +203,7 @@ __global__ void __launch_bounds__(256) int8_values_kernel(const signed char* __r
 
 // A thread a 16-byte piece of the packed matrix; the threads of the first tile of a group see to its scales.
 __global__ void __launch_bounds__(256) int8_pack_kernel(const signed char* __restrict__ values, const float* __restrict__ scales,
-                                                        signed char* __restrict__ packed, float* __restrict__ packed_scales, int n, int stride,
+                                                        signed char* __restrict__ packed, float* __restrict__ packed_scales, int n, int k, int stride,
                                                         long pieces, int gated) {
     const long id = (long)blockIdx.x * blockDim.x + threadIdx.x;
     if (id >= pieces) return;
@@ -214,9 +214,17 @@ __global__ void __launch_bounds__(256) int8_pack_kernel(const signed char* __res
     const bool there = row < n;
     if (gated && within >= 8) row += n;
     const long column = tile % tiles * 64 + lane / 16 * 16;
-    uint4 piece = make_uint4(0u, 0u, 0u, 0u);
-    if (there) piece = *reinterpret_cast<const uint4*>(values + row * stride + column);
-    *reinterpret_cast<uint4*>(packed + id * 16) = piece;
+    unsigned piece[4] = {0u, 0u, 0u, 0u};
+    if (there) {
+        const uint4 read = *reinterpret_cast<const uint4*>(values + row * stride + column);
+        piece[0] = read.x, piece[1] = read.y, piece[2] = read.z, piece[3] = read.w;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {                           // zeros behind the k columns, whatever stood there: what rows hold there then does not count
+            const long left = (long)k - column - i * 4;
+            if (left < 4) piece[i] = left <= 0 ? 0u : piece[i] & ((1u << (left * 8)) - 1u);
+        }
+    }
+    *reinterpret_cast<uint4*>(packed + id * 16) = make_uint4(piece[0], piece[1], piece[2], piece[3]);
     if (tile % tiles == 0 && lane < 16) packed_scales[group * 16 + within] = there ? scales[row] : 0.f;
 }
 
@@ -231,6 +239,7 @@ extern "C" long xrt_int8_packed_rows(int n, int gated) { return int8_groups(n, g
 extern "C" int xrt_quantize_int8(const void* x, int dtype, long x_stride, void* values, float* scales, int rows, int k, void* stream) {
     XRT_REQUIRE(rows >= 0 && k > 0 && k <= XRT_INT8_MOST_K && (rows == 0 || (x && values && scales)), "quantize_int8: bad operands rows=%d k=%d", rows, k);
     XRT_REQUIRE(dtype == XRT_F32 || dtype == XRT_BF16, "quantize_int8: unknown dtype %d", dtype);
+    XRT_REQUIRE((uintptr_t)values % 16 == 0, "quantize_int8: values start at a multiple of 16 bytes");
     XRT_REQUIRE(x_stride >= k, "quantize_int8: rows of %d elements %ld apart", k, x_stride);
     if (rows == 0) return 0;
     const int stride = (int)int8_stride(k);
@@ -253,8 +262,9 @@ extern "C" int xrt_rmsnorm_int8(float* x, const void* delta, int delta_dtype, co
                 "rmsnorm_int8: bad operands rows=%d hidden=%d", n_rows, hidden);
     XRT_REQUIRE((weight_dtype == XRT_F32 || weight_dtype == XRT_BF16) && (!delta || delta_dtype == XRT_F32 || delta_dtype == XRT_BF16),
                 "rmsnorm_int8: unknown dtype weight=%d delta=%d", weight_dtype, delta_dtype);
+    XRT_REQUIRE((uintptr_t)values % 16 == 0, "rmsnorm_int8: values start at a multiple of 16 bytes");
     XRT_REQUIRE(!delta || !rows, "rmsnorm_int8: chosen rows of x cannot be added to (one might be chosen twice)");
-    XRT_REQUIRE(rows || n_rows == x_rows, "rmsnorm_int8: %d rows of results for %d rows of x", n_rows, x_rows);
+    XRT_REQUIRE(n_rows == 0 || rows || n_rows == x_rows, "rmsnorm_int8: %d rows of results for %d rows of x", n_rows, x_rows);
     if (n_rows == 0) return 0;
     const int stride = (int)int8_stride(hidden);
     hipStream_t s = (hipStream_t)stream;
@@ -279,6 +289,7 @@ extern "C" int xrt_rmsnorm_int8(float* x, const void* delta, int delta_dtype, co
 extern "C" int xrt_dequantize_int8(const void* values, const float* scales, void* out, int out_dtype, int rows, int k, void* stream) {
     XRT_REQUIRE(rows >= 0 && k > 0 && k <= XRT_INT8_MOST_K && (rows == 0 || (values && scales && out)), "dequantize_int8: bad operands rows=%d k=%d", rows, k);
     XRT_REQUIRE(out_dtype == XRT_F32 || out_dtype == XRT_BF16, "dequantize_int8: unknown dtype %d", out_dtype);
+    XRT_REQUIRE((uintptr_t)values % 16 == 0, "dequantize_int8: values start at a multiple of 16 bytes");
     if (rows == 0) return 0;
     int lanes = 8;
     while (lanes < 256 && lanes * 8 < k) lanes *= 2;
@@ -293,10 +304,11 @@ extern "C" int xrt_dequantize_int8(const void* values, const float* scales, void
 
 extern "C" int xrt_pack_int8(const void* values, const float* scales, void* packed, float* packed_scales, int n, int k, int gated, void* stream) {
     XRT_REQUIRE(values && scales && packed && packed_scales && n > 0 && k > 0 && k <= XRT_INT8_MOST_K, "pack_int8: bad operands n=%d k=%d", n, k);
+    XRT_REQUIRE(((uintptr_t)values | (uintptr_t)packed) % 16 == 0, "pack_int8: values start at a multiple of 16 bytes");
     const long pieces = int8_groups(n, gated != 0) * int8_stride(k);             // 16 rows of stride bytes, 16 bytes a piece
     const long blocks = (pieces + 255) / 256;
     XRT_REQUIRE(blocks < (1L << 31), "pack_int8: too many elements");
-    int8_pack_kernel<<<(unsigned)blocks, 256, 0, (hipStream_t)stream>>>((const signed char*)values, scales, (signed char*)packed, packed_scales, n,
+    int8_pack_kernel<<<(unsigned)blocks, 256, 0, (hipStream_t)stream>>>((const signed char*)values, scales, (signed char*)packed, packed_scales, n, k,
                                                                         (int)int8_stride(k), pieces, gated != 0);
     XRT_LAUNCH_CHECK("pack_int8");
     return 0;

@@ -108,8 +108,8 @@ int xrt_linear_static(const void* a, const void* w, int dtype, void* out, int ou
                       int mode, void* stream);
 
 // ---- rows and weight matrices in 8-bit integers with scales (csrc/int8.h says how they lie) ----
-// Row m of k columns is values[m][0 .. xrt_int8_stride(k)), signed bytes with zeros from column k on, times scales[m] (float32). values start at a
-// multiple of 16 bytes. k is at most XRT_INT8_K_LIMIT, so that sums of products are exact in 32 bits.
+// Row m of k columns is values[m][0 .. xrt_int8_stride(k)), signed bytes, times scales[m] (float32); from column k on the operators write zeros and read
+// nothing that counts. values start at a multiple of 16 bytes. k is at most XRT_INT8_K_LIMIT, so that sums of products are exact in 32 bits.
 #define XRT_INT8_K_LIMIT 131071
 long xrt_int8_stride(int k);
 // scales[m] = max |x[m]| / 127, values = x / scale rounded to the nearest integer, halves to even; x (float32 or bfloat16) has its rows x_stride

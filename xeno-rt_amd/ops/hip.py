@@ -115,9 +115,9 @@ INT8_MOST_K = 131071        # columns of which a sum of products still fits 32 b
 
 
 class Int8Rows:
-    """Rows in 8-bit integers: row m stands for values[m, :k] * scales[m]. values is int8 [rows, k filled up to a multiple of INT8_STEP], with zeros
-    behind the k columns; scales float32 [rows]. `int8_rows` makes an empty one; `quantize_int8` and `rmsnorm_int8` fill it, `linear_int8` and
-    `linear_glu_int8` multiply it. Whoever fills one in another way keeps the zeros. The tensors are checked here, once, and stay what they are."""
+    """Rows in 8-bit integers: row m stands for values[m, :k] * scales[m]. values is int8 [rows, k filled up to a multiple of INT8_STEP] (what lies behind the
+    k columns does not count), scales float32 [rows]. `int8_rows` makes an empty one; `quantize_int8` and `rmsnorm_int8` fill it, `linear_int8` and
+    `linear_glu_int8` multiply it. The tensors are checked here, once, and stay what they are."""
 
     __slots__ = ("_values", "_scales", "_k", "shape", "index")
 
@@ -155,7 +155,15 @@ class Int8Matrix:
     __slots__ = ("data", "scales", "shape", "gated", "index")
 
     def __init__(self, data: torch.Tensor, scales: torch.Tensor, rows: int, k: int, gated: bool):
-        self.data, self.scales, self.shape, self.gated, self.index = data, scales, (rows, k), gated, data.get_device()
+        n = rows // 2 if gated else rows
+        packed_rows = (n + 7) // 8 * 16 if gated else (n + 15) // 16 * 16
+        if not 0 < k <= INT8_MOST_K or n < 1 or (gated and rows % 2 != 0):
+            raise KernelError(f"weights in 8 bits: {rows} rows of {k} columns")
+        HipOps._require(data, "8-bit weights", torch.int8, (packed_rows, (k + INT8_STEP - 1) // INT8_STEP * INT8_STEP))
+        HipOps._require(scales, "scales of 8-bit weights", torch.float32, (packed_rows,), data)
+        if data.data_ptr() % 16 != 0 or scales.data_ptr() % 16 != 0:
+            raise KernelError("8-bit weights and their scales must start at multiples of 16 bytes")
+        self.data, self.scales, self.shape, self.gated, self.index = data, scales, (int(rows), int(k)), bool(gated), data.get_device()
 
     @property
     def device(self):
