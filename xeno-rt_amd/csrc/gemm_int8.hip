@@ -59,7 +59,11 @@ __device__ __forceinline__ void store_run(TO* out, long m, long n, int M, int N,
     store_run<TO, 4>(out, m, n, M, N, run);
 }
 
-__device__ __forceinline__ float scaled(int sum, float a_scale, float w_scale) { return (float)sum * a_scale * w_scale; }
+// (Not contracted with an addition behind it, which one kernel would do and another not: the bits would go by the number of rows.)
+__device__ __forceinline__ float scaled(int sum, float a_scale, float w_scale) {
+#pragma clang fp contract(off)
+    return (float)sum * a_scale * w_scale;
+}
 
 // What a product writes, and what the sums are multiplied by.
 template <typename TO>
