@@ -195,7 +195,9 @@ SIZES = [(1, 1, 1), (1, 5, 64), (2, 16, 65), (3, 17, 127), (1, 4096, 4096), (5, 
          (64, 257, 2048), (65, 640, 1024), (100, 1001, 777), (128, 128, 128), (129, 255, 300), (200, 3000, 512), (255, 256, 64), (256, 256, 640), (257, 513, 1280), (333, 1280, 5120),
          (512, 6144, 1024), (777, 1001, 2049), (1030, 2050, 384), (2048, 512, 2048), (9, 40000, 128), (300, 24, 9000),
          # 17 to 32 rows of many channels; the larger tiles, with rows and channels that do not fill the last one, one step along k and an odd number of them
-         (20, 16400, 256), (300, 16000, 640), (500, 9000, 500), (1200, 8200, 256), (190, 40000, 100), (70, 5000, 8000), (2049, 7000, 384), (3333, 4111, 120), (800, 12345, 128), (1030, 20000, 128), (10, 100, 9000), (25, 3000, 200)]
+         (20, 16400, 256), (300, 16000, 640), (500, 9000, 500), (1200, 8200, 256), (190, 40000, 100), (70, 5000, 8000), (2049, 7000, 384), (3333, 4111, 120), (800, 12345, 128), (1030, 20000, 128), (10, 100, 9000), (25, 3000, 200),
+         # the narrow tiles, k whole and in two parts
+         (416, 3410, 987), (375, 3418, 4200), (281, 4494, 5951)]
 
 
 @pytest.mark.parametrize("m,n,k", SIZES)

@@ -538,7 +538,9 @@ Plan plan_of(long M, long groups, long stride) {
         Plan plan{0, 0, M <= 16 ? 1 : M <= 32 ? 2 : 4, M <= 16 ? 1 : M <= 32 && groups < 4 * XRT_COMPUTE_UNITS ? 2 : 4, 1};
         const long workgroups = (M + plan.blocks * 16 - 1) / (plan.blocks * 16) * ((groups + plan.groups - 1) / plan.groups);
         const long most = plan.blocks == 1 ? XRT_COMPUTE_UNITS / 2 : XRT_COMPUTE_UNITS;
-        while (plan.parts < 8 && workgroups * plan.parts * 2 <= most && units / (plan.parts * 2) >= 4) plan.parts *= 2;
+        // (64 units of 128 columns by 16 rows at least to begin with, and 16 a part: below, the kernel that adds the parts costs more than they save. 7 rows, k = 926, 297 channels
+        // 2.8 us whole, 4.6 in two; 14, 2108, 74 4.0 and 5.1; 26, 907, 163 3.3 and 4.8; 16, 9000, 512 8.0 whole, 6.9 in four, 7.1 in eight; 73, 9913, 137 24.9 and 9.8 in eight.)
+        while (plan.parts < 8 && workgroups * plan.parts * 2 <= most && units * plan.blocks >= 64 && units * plan.blocks >= plan.parts * 2 * 16) plan.parts *= 2;
         if (M <= 64 || (workgroups <= XRT_COMPUTE_UNITS && units <= (plan.parts == 1 ? 56 : 40 * plan.parts))) return plan;
     }
     // What a tile height costs, fitted to products of 4096 rows, k = 4096 and 14336 (us): a step along k (256 rows: 1.31, 128: 0.80), and the first loads and the
@@ -556,8 +558,10 @@ Plan plan_of(long M, long groups, long stride) {
     long tiles = (M + plan.tile - 1) / plan.tile * tiles_n;
     // Tiles half as wide where the others fill up to half of the chip, and k in parts as far as every compute unit gets one at most: a compute unit pulls no more
     // than some 29 GB/s of w, however much is asked for ahead (100 rows, k = 4096, 14336 pairs 34.5 us in 112 tiles, 28.7 in 224; three steps in LDS instead of two changed nothing).
+    // A step along k takes 0.5 us, the parts' sums and the kernel that adds them 6 to 8, so a short k stays whole (416 rows, k = 987, 1705 pairs 8.9 us whole, 15.1 in two
+    // parts; 423, 2293, 3037 channels 17.7 and 19.2; 375, 6572, 1709 pairs 33.2 and 25.4).
     if (plan.tile == 128 && tiles * 2 <= XRT_COMPUTE_UNITS) plan.width = 128, tiles = (M + 127) / 128 * ((groups + 7) / 8);
-    while (plan.width == 128 && plan.parts < 16 && tiles * plan.parts * 2 <= XRT_COMPUTE_UNITS && units / (plan.parts * 2) >= 3) plan.parts *= 2;
+    while (plan.width == 128 && plan.parts < 16 && tiles * plan.parts * 2 <= XRT_COMPUTE_UNITS && units >= 32) plan.parts *= 2;
     const long steps = (units + plan.parts - 1) / plan.parts;
     plan.parts = (int)((units + steps - 1) / steps);           // (none is empty)
     return plan;
