@@ -438,7 +438,7 @@ def test_refusals(ops):
         lambda: ops.linear_int8(q, w, rand(4, 20).bfloat16(), accumulate=True), lambda: ops.linear_int8(q, w, rand(4, 20).half()),
         lambda: ops.linear_int8(q, w, rand(4, 40)[:, ::2]), lambda: Int8Rows(q.values[:, :100], q.scales, 100), lambda: Int8Rows(q.values.cpu(), q.scales, 100), lambda: Int8Rows(q.values[0], q.scales, 100), lambda: Int8Rows(q.values, q.scales, 129),
         lambda: Int8Rows(q.values.view(-1)[:-1].clone(), q.scales, 100), lambda: Int8Rows(torch.empty(4 * 128 + 8, dtype=torch.int8, device=DEV)[8:].view(4, 128), q.scales, 100),
-        lambda: Int8Rows(q.values, q.scales[:3], 100), lambda: Int8Rows(q.values, q.scales.cpu(), 100), lambda: Int8Rows(q.values, q.scales, 0),
+        lambda: Int8Rows([1, 2], q.scales, 100), lambda: Int8Rows(q.values, q.scales[:3], 100), lambda: Int8Rows(q.values, q.scales.cpu(), 100), lambda: Int8Rows(q.values, q.scales, 0),
         lambda: Int8Matrix(w.data, w.scales, 20, 129, False), lambda: Int8Matrix(w.data, w.scales, 33, 100, False), lambda: Int8Matrix(w.data, w.scales[:8], 20, 100, False),
         lambda: Int8Matrix(w.data.view(torch.uint8), w.scales, 20, 100, False), lambda: Int8Matrix(gated.data, gated.scales, 21, 100, True),
         lambda: ops.rmsnorm_int8(x, gain, EPS, x), lambda: ops.linear_int8(Int8Rows(q.values, q.scales, 101), w, rand(4, 20)),

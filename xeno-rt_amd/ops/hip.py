@@ -122,7 +122,7 @@ class Int8Rows:
     __slots__ = ("_values", "_scales", "_k", "shape", "index")
 
     def __init__(self, values: torch.Tensor, scales: torch.Tensor, k: int):
-        rows, k = values.shape[0] if values.dim() == 2 else -1, int(k)
+        rows, k = values.shape[0] if isinstance(values, torch.Tensor) and values.dim() == 2 else -1, int(k)
         if not 0 < k <= INT8_MOST_K:
             raise KernelError(f"rows in 8 bits: {k} columns, expected 1 to {INT8_MOST_K}")
         HipOps._require(values, "8-bit values", torch.int8, (rows, (k + INT8_STEP - 1) // INT8_STEP * INT8_STEP))
@@ -150,9 +150,9 @@ class Int8Rows:
 
 class Int8Matrix:
     """A weight matrix [rows, k] in 8-bit integers with a scale for each row (output channel), in the tiles in which the products take it
-    (csrc/int8.h). gated: [gate rows | up rows], for `linear_glu_int8`. Made by `pack_int8`."""
+    (csrc/int8.h). gated: [gate rows | up rows], for `linear_glu_int8`. Made by `pack_int8`. The tensors are checked here, once, and stay what they are."""
 
-    __slots__ = ("data", "scales", "shape", "gated", "index")
+    __slots__ = ("_data", "_scales", "shape", "gated", "index")
 
     def __init__(self, data: torch.Tensor, scales: torch.Tensor, rows: int, k: int, gated: bool):
         n = rows // 2 if gated else rows
@@ -163,11 +163,19 @@ class Int8Matrix:
         HipOps._require(scales, "scales of 8-bit weights", torch.float32, (packed_rows,), data)
         if data.data_ptr() % 16 != 0 or scales.data_ptr() % 16 != 0:
             raise KernelError("8-bit weights and their scales must start at multiples of 16 bytes")
-        self.data, self.scales, self.shape, self.gated, self.index = data, scales, (int(rows), int(k)), bool(gated), data.get_device()
+        self._data, self._scales, self.shape, self.gated, self.index = data, scales, (int(rows), int(k)), bool(gated), data.get_device()
+
+    @property
+    def data(self) -> torch.Tensor:
+        return self._data
+
+    @property
+    def scales(self) -> torch.Tensor:
+        return self._scales
 
     @property
     def device(self):
-        return self.data.device
+        return self._data.device
 
     def dim(self) -> int:
         return 2
@@ -716,7 +724,7 @@ class HipOps:
         stream = self._int8_stream(index)
         need = self.lib.xrt_linear_int8_workspace(m, n, k, mode)
         workspace = self._empty(need // 4, torch.int32, out.device) if need > 0 else None
-        status = self.lib.xrt_linear_int8(a._values.data_ptr(), a._scales.data_ptr(), w.data.data_ptr(), w.scales.data_ptr(), at_out, code, m, n, k, mode,
+        status = self.lib.xrt_linear_int8(a._values.data_ptr(), a._scales.data_ptr(), w._data.data_ptr(), w._scales.data_ptr(), at_out, code, m, n, k, mode,
                                           None if workspace is None else workspace.data_ptr(), need, stream)
         if status != 0:
             self._check(status)
