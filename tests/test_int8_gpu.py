@@ -262,6 +262,34 @@ def test_the_largest_sums_are_exact(ops):
         assert bool((out == float(torch.tensor(2 ** 14 * INT8_MOST_K, dtype=torch.float32))).all())
 
 
+# rows, weights and a result of more than 2^31 bytes or elements: what lies last is made from what belongs to it
+def test_offsets_that_pass_32_bits(ops):
+    from xeno_rt_amd.ops.hip import Int8Rows
+    picked = lambda rows, which: Int8Rows(rows.values[which].contiguous(), rows.scales[which].contiguous(), rows.k)          # noqa: E731
+    long, short = whole_numbers(36000, 65536, seed=1), whole_numbers(24, 65536, seed=2)
+    some = torch.tensor([0, 1, 17000, 32767, 32768, 35983, 35998, 35999], device=DEV)
+    some_long = picked(long, some)
+    out = torch.empty(36000, 24, device=DEV)
+    ops.linear_int8(long, ops.pack_int8(short), out)
+    assert near(out[some], exact_product(some_long, short))
+    few, out = picked(short, torch.arange(5, device=DEV)), torch.empty(5, 36000, device=DEV)
+    ops.linear_int8(few, ops.pack_int8(long), out)
+    assert near(out[:, some], exact_product(few, some_long))
+    x = torch.empty(36000, 65536, device=DEV)
+    ops.dequantize_int8(long, x)
+    assert torch.equal(x[some], some_long.values.float() * some_long.scales[:, None])
+    again = ops.int8_rows(36000, 65536, DEV)
+    ops.quantize_int8(x, again)
+    values, scales = plain_rows(x[some])
+    assert torch.equal(again.values[some].float(), values) and torch.equal(again.scales[some], scales)
+    del x, again, long
+    a, w = whole_numbers(20000, 64, seed=3), whole_numbers(110000, 64, seed=4)
+    rows, columns = torch.tensor([0, 12345, 19998, 19999], device=DEV), torch.tensor([0, 1, 65536, 109983, 109999], device=DEV)
+    want, out = exact_product(picked(a, rows), picked(w, columns)), torch.empty(20000, 110000, dtype=torch.bfloat16, device=DEV)
+    ops.linear_int8(a, ops.pack_int8(w), out)
+    assert near(out[rows][:, columns], want)
+
+
 def test_rows_and_channels_without_a_scale(ops):
     """A NaN scale makes its row or its channel NaN and nothing else; a zero scale zeros."""
     for m in (3, 40, 300):

@@ -139,7 +139,8 @@ def sizes(seed, count):
     near = lambda low, high: min(high, max(low, int(round(2 ** spread.uniform(np.log2(low), np.log2(high))))))     # noqa: E731
     for _ in range(count):
         yield near(1, 6000), near(1, 12000), near(1, 20000), spread.choice(list(MODES))
-    for m, n, k in ((1, 1, 1), (1, 1, MOST_K), (300, 17, MOST_K), (64, 20, MOST_K), (65, 9000, 1), (512, 4096, 14336), (512, 6144, 4096), (20000, 300, 100)):
+    for m, n, k in ((1, 1, 1), (1, 1, MOST_K), (300, 17, MOST_K), (64, 20, MOST_K), (65, 9000, 1), (512, 4096, 14336), (512, 6144, 4096), (20000, 300, 100),
+                    (36000, 24, 65536), (5, 36000, 65536), (20000, 110000, 64)):
         yield m, n, k, "add"
 
 
