@@ -26,11 +26,11 @@ def plan_of(lib, m, n, k, mode):
 
 # By registers: up to 16, 32 and 64 rows; few tiles of 64 x 64 above. By LDS: all three heights, the narrow tile, k whole and in parts.
 @pytest.mark.parametrize("m,n,k,mode,plan", [
-    (1, 4096, 4096, "add", (0, 0, 1, 1, 1)), (16, 100, 9000, "store", (0, 0, 1, 1, 4)), (7, 297, 926, "store", (0, 0, 1, 1, 1)), (17, 6144, 4096, "store", (0, 0, 2, 2, 1)), (32, 14336, 4096, "gated", (0, 0, 2, 4, 1)),
-    (33, 14336, 4096, "gated", (0, 0, 4, 4, 1)), (64, 4096, 14336, "add", (0, 0, 4, 4, 4)), (777, 1001, 2049, "store", (0, 0, 4, 4, 1)), (65, 24, 9000, "gated", (0, 0, 4, 4, 8)),
+    (1, 4096, 4096, "add", (0, 0, 1, 1, 1)), (16, 100, 9000, "store", (0, 0, 1, 1, 5)), (7, 297, 926, "store", (0, 0, 1, 1, 1)), (17, 6144, 4096, "store", (0, 0, 2, 2, 1)), (32, 14336, 4096, "gated", (0, 0, 2, 4, 1)),
+    (33, 14336, 4096, "gated", (0, 0, 4, 4, 1)), (64, 4096, 14336, "add", (0, 0, 4, 4, 4)), (777, 1001, 2049, "store", (0, 0, 4, 4, 1)), (65, 24, 9000, "gated", (0, 0, 4, 4, 16)),
     (4096, 4096, 4096, "add", (256, 256, 0, 0, 1)), (4096, 14336, 4096, "gated", (256, 256, 0, 0, 1)), (333, 25600, 5120, "gated", (192, 256, 0, 0, 1)),
     (200, 14336, 4096, "gated", (128, 256, 0, 0, 1)), (128, 14336, 4096, "gated", (128, 128, 0, 0, 1)), (100, 4096, 14336, "add", (128, 128, 0, 0, 8)),
-    (416, 1705, 987, "gated", (128, 128, 0, 0, 1)), (375, 1709, 6572, "gated", (128, 128, 0, 0, 2))])
+    (416, 1705, 987, "gated", (128, 128, 0, 0, 1)), (375, 1709, 6572, "gated", (128, 128, 0, 0, 3))])
 def test_which_kernel_takes_a_product(lib, m, n, k, mode, plan):
     assert tuple(plan_of(lib, m, n, k, mode).values()) == plan
 

@@ -110,9 +110,14 @@ __global__ void __launch_bounds__(256) int8_finish_kernel(const int4v* __restric
     const long block = (long)blockIdx.x * 4 + threadIdx.x / XRT_WAVE;
     if (block >= blocks) return;
     const int4v* at = sums + block * XRT_WAVE + threadIdx.x % XRT_WAVE;
-    int4v sum = at[0];
-#pragma unroll 8
-    for (int p = 1; p < parts; ++p) sum += at[p * blocks * XRT_WAVE];
+    int4v sum{0, 0, 0, 0};
+    for (int first = 0; first < parts; first += 8) {            // eight parts asked for at once, however many there are
+        int4v piece[8];
+#pragma unroll
+        for (int i = 0; i < 8; ++i) piece[i] = first + i < parts ? at[(first + i) * blocks * XRT_WAVE] : int4v{0, 0, 0, 0};
+#pragma unroll
+        for (int i = 0; i < 8; ++i) sum += piece[i];
+    }
     finish_block<MODE, TO>(sum, block / groups * 16, block % groups, to);
 }
 
@@ -538,10 +543,11 @@ Plan plan_of(long M, long groups, long stride) {
         // (two blocks of rows, 1792 groups of w: 27.7 us with two groups a workgroup, 24.5 with four; 384 groups: 9.5 and 11.1)
         Plan plan{0, 0, M <= 16 ? 1 : M <= 32 ? 2 : 4, M <= 16 ? 1 : M <= 32 && groups < 4 * XRT_COMPUTE_UNITS ? 2 : 4, 1};
         const long workgroups = (M + plan.blocks * 16 - 1) / (plan.blocks * 16) * ((groups + plan.groups - 1) / plan.groups);
-        const long most = plan.blocks == 1 ? XRT_COMPUTE_UNITS / 2 : XRT_COMPUTE_UNITS;
-        // (64 units of 128 columns by 16 rows at least to begin with, and 16 a part: below, the kernel that adds the parts costs more than they save. 7 rows, k = 926, 297 channels
-        // 2.8 us whole, 4.6 in two; 14, 2108, 74 4.0 and 5.1; 26, 907, 163 3.3 and 4.8; 16, 9000, 512 8.0 whole, 6.9 in four, 7.1 in eight; 73, 9913, 137 24.9 and 9.8 in eight.)
-        while (plan.parts < 8 && workgroups * plan.parts * 2 <= most && units * plan.blocks >= 64 && units * plan.blocks >= plan.parts * 2 * 16) plan.parts *= 2;
+        // k in as many parts as there are compute units for, each of 12 units of 128 columns by 16 rows at least, if the longest way along k gets shorter by 48 of them:
+        // else the kernel that adds the parts takes what they save. (7 rows, k = 926, 297 channels 2.8 us whole, 4.6 in two; 3, 6640, 538 5.0 and 5.2 in six; 74, 6977, 330
+        // pairs 8.5 in eight, 8.2 in nine; 16, 14336, 1024 11.6 whole, 9.5 in two, 7.7 in four; 239, 14602, 31 9.3 in eight, 7.9 in sixteen.)
+        const int parts = (int)min(min(XRT_COMPUTE_UNITS / workgroups, units * plan.blocks / 12), 16L);
+        if (parts > 1 && units * plan.blocks * (parts - 1) >= 48 * parts) plan.parts = parts;
         if (M <= 64 || (workgroups <= XRT_COMPUTE_UNITS && units <= (plan.parts == 1 ? 56 : 40 * plan.parts))) return plan;
     }
     // What a tile height costs, fitted to products of 4096 rows, k = 4096 and 14336 (us): a step along k (256 rows: 1.31, 128: 0.80), and the first loads and the
@@ -560,9 +566,9 @@ Plan plan_of(long M, long groups, long stride) {
     // Tiles half as wide where the others fill up to half of the chip, and k in parts as far as every compute unit gets one at most: a compute unit pulls no more
     // than some 29 GB/s of w, however much is asked for ahead (100 rows, k = 4096, 14336 pairs 34.5 us in 112 tiles, 28.7 in 224; three steps in LDS instead of two changed nothing).
     // A step along k takes 0.5 us, the parts' sums and the kernel that adds them 6 to 8, so a short k stays whole (416 rows, k = 987, 1705 pairs 8.9 us whole, 15.1 in two
-    // parts; 423, 2293, 3037 channels 17.7 and 19.2; 375, 6572, 1709 pairs 33.2 and 25.4).
+    // parts; 423, 2293, 3037 channels 17.7 and 19.2; 375, 6572, 1709 pairs 33.2 and 25.4; 598, 10587, 851 pairs 31.6 in two, 26.2 in three).
     if (plan.tile == 128 && tiles * 2 <= XRT_COMPUTE_UNITS) plan.width = 128, tiles = (M + 127) / 128 * ((groups + 7) / 8);
-    while (plan.width == 128 && plan.parts < 16 && tiles * plan.parts * 2 <= XRT_COMPUTE_UNITS && units >= 32) plan.parts *= 2;
+    if (plan.width == 128 && units >= 32) plan.parts = (int)max(1L, min(XRT_COMPUTE_UNITS / tiles, 16L));
     const long steps = (units + plan.parts - 1) / plan.parts;
     plan.parts = (int)((units + steps - 1) / steps);           // (none is empty)
     return plan;
