@@ -536,9 +536,10 @@ struct Plan {
 
 Plan plan_of(long M, long groups, long stride) {
     const long units = stride / XRT_INT8_STEP;
-    // The kernel of few rows: up to 64, and more where its tiles of 64 x 64 find a compute unit each and no workgroup goes through more than 7168 columns (5120 of a
-    // k in parts; a tile reads as much of a as of w). It takes a half to nine tenths of the time of the larger tiles there (217 rows, k = 384, 1312 channels 6.9 -> 4.5 us;
-    // 447, 1536, 1440 14.0 -> 7.6; 456, 7168, 912 pairs 23.7 -> 21.0; 239, 7552, 1496 pairs 20.9 -> 22.7; 100, 14336, 4096 channels 22.4 in eight parts, 26.1 in two).
+    // The kernel of few rows: up to 64, and more where its tiles of 64 x 64 find a compute unit each and no workgroup goes through many columns: a tile reads as much
+    // of a as of w, and the larger tiles get k in the more parts the fewer of these there are. Without a cut 40 units of 128 columns to 56 of them by the number of
+    // workgroups (us, and of the larger tiles: 217 rows, k = 384, 1312 channels 4.5 and 6.9; 1233, 5342, 497 15.7 and 17.9; 119, 5724, 4235 19.6 and 15.5; 225, 6021, 4037
+    // 18.4 and 18.7; 92, 8327, 4784 23.4 and 16.4), else 32 a part (144, 15612, 928 14.1 and 15.4; 256, 13719, 1101 19.2 and 17.7; 480, 16494, 975 26.0 and 21.8).
     {
         // (two blocks of rows, 1792 groups of w: 27.7 us with two groups a workgroup, 24.5 with four; 384 groups: 9.5 and 11.1)
         Plan plan{0, 0, M <= 16 ? 1 : M <= 32 ? 2 : 4, M <= 16 ? 1 : M <= 32 && groups < 4 * XRT_COMPUTE_UNITS ? 2 : 4, 1};
@@ -548,7 +549,7 @@ Plan plan_of(long M, long groups, long stride) {
         // pairs 8.5 in eight, 8.2 in nine; 16, 14336, 1024 11.6 whole, 9.5 in two, 7.7 in four; 239, 14602, 31 9.3 in eight, 7.9 in sixteen.)
         const int parts = (int)min(min(XRT_COMPUTE_UNITS / workgroups, units * plan.blocks / 12), 16L);
         if (parts > 1 && units * plan.blocks * (parts - 1) >= 48 * parts) plan.parts = parts;
-        if (M <= 64 || (workgroups <= XRT_COMPUTE_UNITS && units <= (plan.parts == 1 ? 56 : 40 * plan.parts))) return plan;
+        if (M <= 64 || (workgroups <= XRT_COMPUTE_UNITS && units <= (plan.parts == 1 ? 24 + workgroups / 8 : 32 * plan.parts))) return plan;
     }
     // What a tile height costs, fitted to products of 4096 rows, k = 4096 and 14336 (us): a step along k (256 rows: 1.31, 128: 0.80), and the first loads and the
     // epilogue. A partly filled round takes half of a full one and its share of the rest: power bounds the chip, and the compute units at work run faster.
