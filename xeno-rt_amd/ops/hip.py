@@ -640,11 +640,12 @@ class HipOps:
         return tensor.data_ptr()
 
     def int8_rows(self, rows: int, k: int, device) -> Int8Rows:
-        """Room for `rows` rows of k columns in 8-bit integers; what it holds is not defined."""
+        """Room for `rows` rows of k columns in 8-bit integers; what it holds is not defined. It is the caller's to keep: torch's memory, also while a step
+        of an engine runs, whose own memory the next step starts over with."""
         if rows < 0 or not 0 < k <= INT8_MOST_K:
             raise KernelError(f"int8_rows: {rows} rows of {k} columns; up to {INT8_MOST_K} columns are possible")
-        return Int8Rows(self._empty((rows, (k + INT8_STEP - 1) // INT8_STEP * INT8_STEP), torch.int8, device),
-                        self._empty((rows,), torch.float32, device), k)
+        return Int8Rows(torch.empty((rows, (k + INT8_STEP - 1) // INT8_STEP * INT8_STEP), dtype=torch.int8, device=device),
+                        torch.empty((rows,), dtype=torch.float32, device=device), k)
 
     def quantize_int8(self, x, out: Int8Rows):
         """out = the rows of x (float32 or bfloat16, some columns of a wider matrix will do) in 8-bit integers: scales[m] = max |x[m]| / 127, values =
@@ -723,7 +724,8 @@ class HipOps:
             raise KernelError(f"linear_int8 out: added to in {out.dtype}, expected float32")
         stream = self._int8_stream(index)
         need = self.lib.xrt_linear_int8_workspace(m, n, k, mode)
-        workspace = self._empty(need // 4, torch.int32, out.device) if need > 0 else None
+        # (torch's memory, never a running step's: this call may come from another thread, on a stream that is not the step's)
+        workspace = torch.empty(need // 4, dtype=torch.int32, device=out.device) if need > 0 else None
         status = self.lib.xrt_linear_int8(a._values.data_ptr(), a._scales.data_ptr(), w._data.data_ptr(), w._scales.data_ptr(), at_out, code, m, n, k, mode,
                                           None if workspace is None else workspace.data_ptr(), need, stream)
         if status != 0:
