@@ -26,7 +26,7 @@ struct Arena {
     void* take(long bytes) {                                    // (a plan's pointers are never followed; they are aligned like the real ones)
         char* p = (plan ? (char*)256 : base) + at;
         at += (bytes + 255) / 256 * 256;
-        most = max(most, at);
+        most = std::max(most, at);                              // (max by itself is one of two ints in host code: from 2^31 bytes on it forgets them)
         return p;
     }
 };
