@@ -11,10 +11,13 @@
 // Up to 64 rows the product is bound by reading w, and gemm_int8_few_kernel streams it through registers. More rows go through tiles in LDS
 // (gemm_int8_large_kernel). Where there are too few workgroups for the chip, k is cut into parts whose sums, as the lanes hold them, go to a workspace;
 // int8_finish_kernel adds them and does the rest.
+#include <limits.h>
+
+#include <algorithm>
 #include <type_traits>
 #include "int8.h"
 #include "activation.h"
-#include "large_tiles.h"
+#include "int8_places.h"
 
 namespace {
 
@@ -137,37 +140,34 @@ __global__ void __launch_bounds__(WAVES * XRT_WAVE, MT * G <= 2 ? 4 : 2) gemm_in
     __shared__ int4v shared[WAVES][AT_ONCE][XRT_WAVE];
     // An XCD gets a run of tiles; split over one tile of rows: tiles and parts in turn. (8 rows, k = 4096, 1792 groups 20.4 us in runs, 23.2 in turn; 64 rows,
     // k = 14336, 4096 channels in four parts 19.4 and 17.8.)
-    const PartPlace place = PARTS && ONCE ? PartPlace{TilePlace{(int)blockIdx.x < tiles_n * parts ? 0 : -1, (int)blockIdx.x % tiles_n}, (int)blockIdx.x / tiles_n}
-                                          : part_place(blockIdx.x, 0, tiles_m, tiles_n, PARTS ? parts : 0);
+    const PartPlace place = few_place(blockIdx.x, tiles_m, tiles_n, PARTS, parts, ONCE);
     if (place.tile.m < 0) return;
     const int lane = threadIdx.x % XRT_WAVE, wave = __builtin_amdgcn_readfirstlane(threadIdx.x / XRT_WAVE);
-    const int r = lane % 16, c = lane / 16;
     const int first_group = place.tile.n * G, first_block = place.tile.m * MT;
 
-    // units of 128 columns, dealt evenly to the parts and within a part to the wavefronts
-    const int units = stride / XRT_INT8_STEP;
+    // units of 128 columns
     const int part = PARTS ? place.part : 0;
-    const int begin = PARTS ? (int)((long)units * part / parts) : 0, end = PARTS ? (int)((long)units * (part + 1) / parts) : units;
-    const int first = begin + (end - begin) * wave / WAVES, count = begin + (end - begin) * (wave + 1) / WAVES - first;
+    const Share share = few_share(stride / XRT_INT8_STEP, PARTS, part, parts, wave, WAVES);
+    const int first = share.first, count = share.count;
 
     const signed char* w_at[G];
     const signed char* a_at[MT];
 #pragma unroll
-    for (int g = 0; g < G; ++g) w_at[g] = w + (long)min(first_group + g, groups - 1) * 16 * stride + (long)first * 2048 + lane * 16;       // groups beyond the matrix: the last one again
+    for (int g = 0; g < G; ++g) w_at[g] = w + few_w_offset(first_group + g, groups, stride, first, lane);
 #pragma unroll
-    for (int i = 0; i < MT; ++i) a_at[i] = a + (long)min((first_block + i) * 16 + r, M - 1) * stride + (long)first * 128 + c * 16;         // rows likewise
+    for (int i = 0; i < MT; ++i) a_at[i] = a + few_a_offset(first_block + i, M, stride, first, lane);
 
     struct Unit { int4v w[G][2], a[MT][2]; };
     auto load = [&](Unit& unit, int u) {
 #pragma unroll
         for (int i = 0; i < MT; ++i)
 #pragma unroll
-            for (int j = 0; j < 2; ++j) unit.a[i][j] = *reinterpret_cast<const int4v*>(a_at[i] + (long)u * 128 + j * 64);
+            for (int j = 0; j < 2; ++j) unit.a[i][j] = *reinterpret_cast<const int4v*>(a_at[i] + (long)u * STEP_A + j * (STEP_A / 2));
 #pragma unroll
         for (int g = 0; g < G; ++g)
 #pragma unroll
             for (int j = 0; j < 2; ++j) {
-                const int4v* from = reinterpret_cast<const int4v*>(w_at[g] + (long)u * 2048 + j * 1024);
+                const int4v* from = reinterpret_cast<const int4v*>(w_at[g] + (long)u * STEP_W + j * (STEP_W / 2));
                 unit.w[g][j] = ONCE ? __builtin_nontemporal_load(from) : *from;
             }
     };
@@ -221,7 +221,7 @@ __global__ void __launch_bounds__(WAVES * XRT_WAVE, MT * G <= 2 ? 4 : 2) gemm_in
         for (int other = 1; other < WAVES; ++other) sum += shared[other][wave][lane];
         const int group = first_group + (t0 + wave) / MT, block = first_block + (t0 + wave) % MT;
         if (group >= groups || block * 16 >= M) continue;
-        if constexpr (PARTS) sums[(((long)part * ((M + 15) / 16) + block) * groups + group) * XRT_WAVE + lane] = sum;
+        if constexpr (PARTS) sums[sums_place(part, M, block, groups, group) + lane] = sum;
         else finish_block<MODE, TO>(sum, (long)block * 16, group, to);
     }
 }
@@ -242,7 +242,7 @@ template <int BM, int BN, int MODE, typename TO, bool PARTS>
 __global__ void __launch_bounds__(8 * XRT_WAVE) gemm_int8_large_kernel(const signed char* __restrict__ a, const signed char* __restrict__ w, int4v* __restrict__ sums,
                                                                        int stride, int groups, int tiles_m, int tiles_n, int height, int by_parts,
                                                                        int steps_a_part, const Result<TO> to) {
-    constexpr int STEP = XRT_INT8_STEP, WAVES_N = 4;
+    constexpr int STEP = XRT_INT8_STEP, WAVES_N = LARGE_WAVES_N;
     constexpr int WAVE_M = BM / 2, WAVE_N = BN / WAVES_N;      // the wavefront's part of the tile
     constexpr int TM = WAVE_M / 16, TN = WAVE_N / 16, HM = TM / 2, HN = TN / 2;      // blocks of 16 rows of a and of w: all, and a half
     constexpr int BLOCKS_A = BM / 16;                          // kilobytes of one half of a: where they do not divide among the wavefronts, the spare loads fetch the last one again
@@ -256,55 +256,45 @@ __global__ void __launch_bounds__(8 * XRT_WAVE) gemm_int8_large_kernel(const sig
     const PartPlace dealt = PARTS ? part_place(blockIdx.x, blockIdx.y, tiles_m, tiles_n, by_parts) : PartPlace{tile_place(blockIdx.x, tiles_m, tiles_n), 0};
     if (dealt.tile.m < 0) return;
     const int M = to.M, N = to.N;
-    const int m0 = dealt.tile.m * height, first_group = dealt.tile.n * (BN / 16);
     const int lane = threadIdx.x % XRT_WAVE, wave = __builtin_amdgcn_readfirstlane(threadIdx.x / XRT_WAVE);
     const int wave_m = wave / WAVES_N, wave_n = wave % WAVES_N;
     const int quad = lane / 16;                                // which four packed rows of a block this lane has the sums of
-    const int upper_blocks = (height / 16 + 1) / 2;            // of 16 rows, of the wavefronts 0 to 3
-    const int blocks = wave_m == 0 ? upper_blocks : height / 16 - upper_blocks;
-    const int wave_row = m0 + wave_m * upper_blocks * 16, tile_end = min(m0 + height, M);
-    a += (long)m0 * stride;                                    // (offsets inside a tile fit 32 bits: 256 rows of up to 131072 bytes)
+    const LargeTile tile = large_tile(dealt.tile, BM, BN, height, M, wave);
+    const int m0 = tile.m0, first_group = tile.first_group, blocks = tile.blocks, wave_row = tile.wave_row;
+    a += (long)m0 * stride;
     w += (long)first_group * 16 * stride;
 
-    // Piece c (16 bytes) of row r lies at place c ^ (r % 8) of the row: the lanes that a 16-byte read serves at once then take different banks.
-    // The kilobyte of LDS (8 rows of a, or a packed tile) that load i of half h fills, for a wavefront; rows: a wavefront's rows of the operand in the tile.
-    auto block_of = [&](int h, int i, int rows, int blocks) {
-        const int per = rows / 16, p = min(i * 8 + wave, blocks - 1);
-        return (p / per * rows + h * (rows / 2)) / 8 + p % per;
-    };
+    // (The pieces of a row of a change places: the lanes that a 16-byte read serves at once then take different banks.)
+    auto block_of = [&](int h, int i, int rows, int blocks) { return large_block(h, i, rows, blocks, wave); };
     unsigned off_a[2][LOADS_A], off_b[2][LOADS_B];             // bytes
-    const int missing = WAVE_M - upper_blocks * 16;            // (rows of the tile that no wavefront has: the last one again, not multiplied)
-    const unsigned piece_of_lane = (unsigned)((lane % 8) ^ (lane / 8)) * 16u;
 #pragma unroll
     for (int h = 0; h < 2; ++h)
 #pragma unroll
-        for (int i = 0; i < LOADS_A; ++i) {
-            const int block = block_of(h, i, WAVE_M, BLOCKS_A), row = block * 8 + lane / 8 - (block * 8 >= WAVE_M ? missing : 0);
-            off_a[h][i] = (unsigned)min(row, tile_end - 1 - m0) * (unsigned)stride + piece_of_lane;
-        }
+        for (int i = 0; i < LOADS_A; ++i) off_a[h][i] = large_a_offset(tile, block_of(h, i, WAVE_M, BLOCKS_A), BM, stride, lane);
 #pragma unroll
     for (int h = 0; h < 2; ++h)
 #pragma unroll
-        for (int i = 0; i < LOADS_B; ++i) {
-            const int block = block_of(h, i, WAVE_N, BN / 16);
-            const int group = min(block / 2, groups - 1 - first_group);                    // groups beyond the matrix: the last one again
-            off_b[h][i] = (unsigned)group * 16u * (unsigned)stride + (unsigned)(block % 2) * 1024u + (unsigned)lane * 16u;
-        }
+        for (int i = 0; i < LOADS_B; ++i) off_b[h][i] = large_w_offset(tile, block_of(h, i, WAVE_N, BN / 16), groups, stride, lane);
     const unsigned lds_a0 = lds_address(stage_a), lds_b0 = lds_address(stage_b);
     auto issue_a = [&](int h, int stage, int step) {
 #pragma unroll
         for (int i = 0; i < LOADS_A; ++i)
-            load_to_lds(a, off_a[h][i] + (unsigned)step * 128u, lds_a0 + (unsigned)(stage * BM * STEP + block_of(h, i, WAVE_M, BLOCKS_A) * 1024));
+            load_to_lds(a, off_a[h][i] + (unsigned)step * (unsigned)STEP_A, lds_a0 + (unsigned)(stage * BM * STEP + block_of(h, i, WAVE_M, BLOCKS_A) * 1024));
     };
     auto issue_b = [&](int h, int stage, int step) {
 #pragma unroll
         for (int i = 0; i < LOADS_B; ++i)
-            load_to_lds(w, off_b[h][i] + (unsigned)step * 2048u, lds_b0 + (unsigned)(stage * BN * STEP + block_of(h, i, WAVE_N, BN / 16) * 1024));
+            load_to_lds(w, off_b[h][i] + (unsigned)step * (unsigned)STEP_W, lds_b0 + (unsigned)(stage * BN * STEP + block_of(h, i, WAVE_N, BN / 16) * 1024));
     };
     // the tile's scales, ahead of the tiles themselves: wavefronts 0 to 3 those of 64 rows of a each, 4 to 7 those of 64 packed rows of w
     if constexpr (!PARTS) {
-        if (wave < 4) load_dword_to_lds(to.a_scales, (unsigned)min(m0 + wave * 64 + lane, M - 1) * 4u, lds_address(lds_a_scales + wave * 64));
-        else if ((wave - 4) * 64 < BN) load_dword_to_lds(to.w_scales, (unsigned)min(first_group * 16 + (wave - 4) * 64 + lane, groups * 16 - 1) * 4u, lds_address(lds_w_scales + (wave - 4) * 64));
+        if (wave < 4) {
+            const ScalePlace at = large_a_scale(tile, wave * 64 + lane, M);
+            load_dword_to_lds(to.a_scales + at.first, at.offset, lds_address(lds_a_scales + wave * 64));
+        } else if ((wave - 4) * 64 < BN) {
+            const ScalePlace at = large_w_scale(tile, (wave - 4) * 64 + lane, groups);
+            load_dword_to_lds(to.w_scales + at.first, at.offset, lds_address(lds_w_scales + (wave - 4) * 64));
+        }
     }
     // where this lane finds its 16 bytes of block 0 of its wavefront, for either 64 columns of the tile
     const unsigned char* place_a[2];
@@ -347,8 +337,8 @@ __global__ void __launch_bounds__(8 * XRT_WAVE) gemm_int8_large_kernel(const sig
                     if (h * HM + i < T)
                         acc[h * HM + i][g * HN + j] = __builtin_amdgcn_mfma_i32_16x16x64_i8(wb[g][ks][j], xa[h][ks][i], acc[h * HM + i][g * HN + j], 0, 0, 0);
     };
-    const int first_step = dealt.part * steps_a_part;
-    const int steps = min(steps_a_part, stride / STEP - first_step), last_step = first_step + steps - 1;
+    const Share share = large_share(stride / STEP, dealt.part, steps_a_part);
+    const int first_step = share.first, steps = share.count, last_step = first_step + steps - 1;
     auto step_of = [&](int t) { return min(first_step + t, last_step); };        // (tiles beyond the end: the last one again, into a place nobody reads)
 #pragma unroll
     for (int t = 0; t < 2; ++t) {
@@ -399,15 +389,14 @@ __global__ void __launch_bounds__(8 * XRT_WAVE) gemm_int8_large_kernel(const sig
     wait_loads_and_barrier<0>();                               // nothing lands in LDS after this
 
     // ---- epilogue: element e of acc[i][j] is row i * 16 + lane % 16 of a and packed row j * 16 + quad * 4 + e of w
-    const int row_end = min(wave_row + blocks * 16, tile_end);           // of the wavefront's rows
-    const int wave_group = first_group + wave_n * TN;
+    const int row_end = large_row_end(tile), wave_group = tile.wave_group;
     if constexpr (PARTS) {
 #pragma unroll
         for (int i = 0; i < TM; ++i)
 #pragma unroll
             for (int j = 0; j < TN; ++j)
                 if (wave_row + i * 16 < row_end && wave_group + j < groups)
-                    sums[(((long)dealt.part * ((M + 15) / 16) + wave_row / 16 + i) * groups + wave_group + j) * XRT_WAVE + lane] = acc[i][j];
+                    sums[sums_place(dealt.part, M, wave_row / 16 + i, groups, wave_group + j) + lane] = acc[i][j];
         return;
     }
     float4 w_scale[TN];
@@ -649,6 +638,75 @@ extern "C" int xrt_linear_int8_plan(int M, int N, int K, int mode, int* plan) {
     XRT_REQUIRE(plan && M > 0 && N > 0 && K > 0 && K <= XRT_INT8_MOST_K, "linear_int8: bad sizes M=%d N=%d K=%d", M, N, K);
     const Plan chosen = plan_of(M, int8_groups(N, mode_of(mode) == MODE_GATED), int8_stride(K));
     plan[0] = chosen.tile, plan[1] = chosen.width, plan[2] = chosen.blocks, plan[3] = chosen.groups, plan[4] = chosen.parts;
+    return 0;
+}
+
+// What a workgroup of such a product reads and which blocks of the result it makes, by the functions that the kernels call (int8_places.h).
+extern "C" int xrt_linear_int8_reach(int M, int N, int K, int mode, long workgroup, long* reach, int* made, int room) {
+    XRT_REQUIRE(reach && made && M > 0 && N > 0 && K > 0 && K <= XRT_INT8_MOST_K && workgroup >= 0, "linear_int8: bad sizes M=%d N=%d K=%d", M, N, K);
+    const long long_groups = int8_groups(N, mode_of(mode) == MODE_GATED);
+    const Plan plan = plan_of(M, long_groups, int8_stride(K));
+    const int groups = (int)long_groups, stride = (int)int8_stride(K), units = stride / XRT_INT8_STEP;
+    const bool in_lds = plan.tile > 0, once = M <= 64, cut = plan.parts > 1;
+    const int bm = plan.tile, bn = plan.width, height = in_lds ? even_height(M, bm) : plan.blocks * 16, wide = in_lds ? bn / 16 : plan.groups;
+    const int tiles_m = (M + height - 1) / height, tiles_n = (groups + wide - 1) / wide;
+    for (int i = 0; i < 10; ++i) reach[i] = i % 2 == 0 ? LONG_MAX : 0;
+    reach[10] = part_ids((long)tiles_m * tiles_n, plan.parts, true);
+    reach[11] = plan.parts;
+    XRT_REQUIRE(workgroup < reach[10] && reach[10] < (1L << 31), "linear_int8: workgroup %ld of %ld", workgroup, reach[10]);
+    auto reads = [&](int operand, long offset, long size) { reach[2 * operand] = std::min(reach[2 * operand], offset), reach[2 * operand + 1] = std::max(reach[2 * operand + 1], offset + size); };
+    int count = 0;
+    auto makes = [&](int part, int block, int group) {
+        if (cut) reads(4, sums_place(part, M, block, groups, group) * (long)sizeof(int4v), XRT_WAVE * sizeof(int4v));
+        if (count < room) made[3 * count] = part, made[3 * count + 1] = block, made[3 * count + 2] = group;
+        ++count;
+    };
+    const PartPlace at = !in_lds ? few_place((int)workgroup, tiles_m, tiles_n, cut, plan.parts, once)
+                         : cut   ? part_place((int)workgroup, 0, tiles_m, tiles_n, plan.parts)
+                                 : PartPlace{tile_place((int)workgroup, tiles_m, tiles_n), 0};
+    reach[12] = 0;
+    reach[13] = 0;
+    if (at.tile.m < 0) return 0;
+    for (int wave = 0; wave < 8; ++wave) {
+        const Share share = in_lds ? large_share(units, at.part, (units + plan.parts - 1) / plan.parts) : few_share(units, cut, at.part, plan.parts, wave, WAVES);
+        XRT_REQUIRE(share.count >= (in_lds ? 1 : 0) && share.first + share.count <= units, "linear_int8: steps %d to %d of %d", share.first, share.first + share.count, units);
+        if (wave == 0 || !in_lds) reach[12] += share.count;
+        const LargeTile tile = in_lds ? large_tile(at.tile, bm, bn, height, M, wave) : LargeTile{};
+        for (int lane = 0; lane < XRT_WAVE; ++lane) {
+            for (int step : {0, share.count - 1}) {
+                if (step < 0) continue;
+                if (!in_lds) {
+                    for (int half = 0; half < 2; ++half) {
+                        for (int i = 0; i < plan.blocks; ++i) reads(0, few_a_offset(at.tile.m * plan.blocks + i, M, stride, share.first, lane) + (long)step * STEP_A + half * (STEP_A / 2), 16);
+                        for (int g = 0; g < wide; ++g) reads(1, few_w_offset(at.tile.n * wide + g, groups, stride, share.first, lane) + (long)step * STEP_W + half * (STEP_W / 2), 16);
+                    }
+                    continue;
+                }
+                for (int h = 0; h < 2; ++h) {
+                    for (int i = 0; i < (bm / 16 + 7) / 8; ++i)
+                        reads(0, (long)tile.m0 * stride + (large_a_offset(tile, large_block(h, i, bm / 2, bm / 16, wave), bm, stride, lane) + (unsigned)(share.first + step) * (unsigned)STEP_A), 16);
+                    for (int i = 0; i < bn / 128; ++i)
+                        reads(1, (long)tile.first_group * 16 * stride + (large_w_offset(tile, large_block(h, i, bn / LARGE_WAVES_N, bn / 16, wave), groups, stride, lane) + (unsigned)(share.first + step) * (unsigned)STEP_W), 16);
+                }
+            }
+            if (in_lds && !cut && wave < 4) {
+                const ScalePlace scale = large_a_scale(tile, wave * 64 + lane, M);
+                reads(2, scale.first * 4 + scale.offset, 4);
+            } else if (in_lds && !cut && (wave - 4) * 64 < bn) {
+                const ScalePlace scale = large_w_scale(tile, (wave - 4) * 64 + lane, groups);
+                reads(3, scale.first * 4 + scale.offset, 4);
+            }
+        }
+        if (!in_lds) continue;
+        for (int row = tile.wave_row; row < large_row_end(tile); row += 16)
+            for (int j = 0; j < bn / LARGE_WAVES_N / 16; ++j)
+                if (tile.wave_group + j < groups) makes(at.part, row / 16, tile.wave_group + j);
+    }
+    if (!in_lds)
+        for (int i = 0; i < plan.blocks; ++i)
+            for (int g = 0; g < wide; ++g)
+                if ((at.tile.m * plan.blocks + i) * 16 < M && at.tile.n * wide + g < groups) makes(at.part, at.tile.m * plan.blocks + i, at.tile.n * wide + g);
+    reach[13] = count;
     return 0;
 }
 

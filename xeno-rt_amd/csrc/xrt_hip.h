@@ -133,6 +133,12 @@ long xrt_linear_int8_workspace(int M, int N, int K, int mode);
 // What such a product takes, for tests: plan[0], plan[1] the rows of a and the packed rows of w of a tile in LDS (0, 0: it is streamed through registers, plan[2]
 // blocks of 16 rows of a and plan[3] groups of 16 packed rows of w a workgroup), plan[4] the parts that k is cut into.
 int xrt_linear_int8_plan(int M, int N, int K, int mode, int* plan);
+// What one workgroup of such a product's launch reaches, for tests too, worked out on the host by the functions that the kernels call. reach[2 i], reach[2 i + 1]: the
+// first byte and the one behind the last that it reads of a, of w, of a's scales, of w's (both: of tiles in LDS that are not cut, else LONG_MAX and 0) and that it writes
+// of the workspace; reach[10] the launch's workgroups, reach[11] the parts of k, reach[12] the steps of 128 columns that it goes through, reach[13] the blocks (16 rows of a, 16
+// packed rows of w) it makes. made: part, block of rows and group of w of up to `room` of them.
+#define XRT_INT8_REACH 14
+int xrt_linear_int8_reach(int M, int N, int K, int mode, long workgroup, long* reach, int* made, int room);
 
 // An RMSNorm between two products, x += a w^T; y = rmsnorm(x) * gain; z = y v^T, without a kernel of
 // its own. The first product (mode 1) also writes scaled_out[m, n] = bfloat16(x[m, n] * gain[n]) and
