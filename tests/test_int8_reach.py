@@ -81,3 +81,10 @@ def test_every_block_is_made_once_and_every_byte_is_inside(lib, seed):
 @pytest.mark.parametrize("size", ENDS, ids=str)
 def test_the_ends_of_the_range(lib, size):
     check(lib, *size)
+
+
+# 2^30 rows and more of one step along k: a row's scale lies 2^32 bytes and more behind the first one's
+@pytest.mark.parametrize("m", [2 ** 30 - 300, 2 ** 30 + 4096, 2 ** 30 + 2 ** 29 + 77])
+def test_rows_whose_scales_pass_2_to_the_32_bytes(lib, m):
+    middle = 2 ** 30 // 256
+    check(lib, m, 1, 64, "store", lambda workgroups: [0, 1, 7, workgroups // 2, *range(min(middle, workgroups) - 40, min(middle, workgroups)), *range(workgroups - 40, workgroups)])

@@ -80,10 +80,12 @@ __host__ __device__ __forceinline__ unsigned large_w_offset(const LargeTile& t, 
     return (unsigned)min(block / 2, groups - 1 - t.first_group) * 16u * (unsigned)stride + (unsigned)(block % 2) * 1024u + (unsigned)lane * 16u;
 }
 
-// The tile's scales, of row i of a and packed row i of w: from the one at `first` on, bytes.
+// The scales of row i of the tile's rows of a and of its packed row i of w: from the tile's first one on (in 64 bits: 2^30 rows of scales are 2^32 bytes), bytes.
 struct ScalePlace { long first; unsigned offset; };
-__host__ __device__ __forceinline__ ScalePlace large_a_scale(const LargeTile& t, int i, int M) { return ScalePlace{0, (unsigned)min(t.m0 + i, M - 1) * 4u}; }
-__host__ __device__ __forceinline__ ScalePlace large_w_scale(const LargeTile& t, int i, int groups) { return ScalePlace{0, (unsigned)min(t.first_group * 16 + i, groups * 16 - 1) * 4u}; }
+__host__ __device__ __forceinline__ ScalePlace large_a_scale(const LargeTile& t, int i, int M) { return ScalePlace{t.m0, (unsigned)min(i, M - 1 - t.m0) * 4u}; }
+__host__ __device__ __forceinline__ ScalePlace large_w_scale(const LargeTile& t, int i, int groups) {
+    return ScalePlace{(long)t.first_group * 16, (unsigned)min(i, (groups - t.first_group) * 16 - 1) * 4u};
+}
 
 // The steps along k of a part: steps_a_part of them, the last part what is left.
 __host__ __device__ __forceinline__ Share large_share(int units, int part, int steps_a_part) {
