@@ -84,7 +84,15 @@ def test_the_ends_of_the_range(lib, size):
 
 
 # 2^30 rows and more of one step along k: a row's scale lies 2^32 bytes and more behind the first one's
-@pytest.mark.parametrize("m", [2 ** 30 - 300, 2 ** 30 + 4096, 2 ** 30 + 2 ** 29 + 77])
+@pytest.mark.parametrize("m", [2 ** 30 - 300, 2 ** 30 + 4096, 2 ** 30 + 2 ** 29 + 77, 2 ** 31 - 300])
 def test_rows_whose_scales_pass_2_to_the_32_bytes(lib, m):
     middle = 2 ** 30 // 256
     check(lib, m, 1, 64, "store", lambda workgroups: [0, 1, 7, workgroups // 2, *range(min(middle, workgroups) - 40, min(middle, workgroups)), *range(workgroups - 40, workgroups)])
+
+
+def test_more_rows_than_32_bits_number_are_refused(lib):
+    lib.xrt_last_error.restype = ctypes.c_char_p
+    plan, at = (ctypes.c_int * 5)(), ctypes.c_void_p(1 << 20)
+    for m, n, mode in ((2 ** 31 - 1, 1, "store"), (2 ** 31 - 256, 1, "add"), (1, 2 ** 30, "store"), (1, 2 ** 29, "gated"), (4096, 2 ** 31 - 1, "store")):
+        assert lib.xrt_linear_int8_plan(m, n, 64, MODES[mode], plan) != 0 and lib.xrt_linear_int8_workspace(m, n, 64, MODES[mode]) == 0
+        assert lib.xrt_linear_int8(at, at, at, at, at, 0, m, n, 64, MODES[mode], None, ctypes.c_long(0), None) != 0 and b"too many rows" in lib.xrt_last_error()

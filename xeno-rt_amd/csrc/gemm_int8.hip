@@ -628,14 +628,17 @@ int launch(const Operands& o, const Plan& plan, const Result<TO>& to) {
 
 }  // namespace
 
+// Whether row numbers, and a tile's rows behind the last, fit 32 bits, and the packed rows of w (two for an output of a gated matrix) 30.
+static bool sizes_fit(int M, int N, int mode) { return (long)M + 256 < (1L << 31) && int8_groups(N, mode_of(mode) == MODE_GATED) * 16 < (1L << 30); }
+
 extern "C" long xrt_linear_int8_workspace(int M, int N, int K, int mode) {
-    if (M <= 0 || N <= 0 || K <= 0 || K > XRT_INT8_MOST_K) return 0;
+    if (M <= 0 || N <= 0 || K <= 0 || K > XRT_INT8_MOST_K || !sizes_fit(M, N, mode)) return 0;
     const long groups = int8_groups(N, mode_of(mode) == MODE_GATED);
     return sums_bytes(plan_of(M, groups, int8_stride(K)), M, groups);
 }
 
 extern "C" int xrt_linear_int8_plan(int M, int N, int K, int mode, int* plan) {
-    XRT_REQUIRE(plan && M > 0 && N > 0 && K > 0 && K <= XRT_INT8_MOST_K, "linear_int8: bad sizes M=%d N=%d K=%d", M, N, K);
+    XRT_REQUIRE(plan && M > 0 && N > 0 && K > 0 && K <= XRT_INT8_MOST_K && sizes_fit(M, N, mode), "linear_int8: bad sizes M=%d N=%d K=%d", M, N, K);
     const Plan chosen = plan_of(M, int8_groups(N, mode_of(mode) == MODE_GATED), int8_stride(K));
     plan[0] = chosen.tile, plan[1] = chosen.width, plan[2] = chosen.blocks, plan[3] = chosen.groups, plan[4] = chosen.parts;
     return 0;
@@ -643,7 +646,7 @@ extern "C" int xrt_linear_int8_plan(int M, int N, int K, int mode, int* plan) {
 
 // What a workgroup of such a product reads and which blocks of the result it makes, by the functions that the kernels call (int8_places.h).
 extern "C" int xrt_linear_int8_reach(int M, int N, int K, int mode, long workgroup, long* reach, int* made, int room) {
-    XRT_REQUIRE(reach && made && M > 0 && N > 0 && K > 0 && K <= XRT_INT8_MOST_K && workgroup >= 0, "linear_int8: bad sizes M=%d N=%d K=%d", M, N, K);
+    XRT_REQUIRE(reach && made && M > 0 && N > 0 && K > 0 && K <= XRT_INT8_MOST_K && sizes_fit(M, N, mode) && workgroup >= 0, "linear_int8: bad sizes M=%d N=%d K=%d", M, N, K);
     const long long_groups = int8_groups(N, mode_of(mode) == MODE_GATED);
     const Plan plan = plan_of(M, long_groups, int8_stride(K));
     const int groups = (int)long_groups, stride = (int)int8_stride(K), units = stride / XRT_INT8_STEP;
@@ -719,11 +722,11 @@ extern "C" int xrt_linear_int8(const void* a, const float* a_scales, const void*
     XRT_REQUIRE(out_dtype == XRT_F32 || (out_dtype == XRT_BF16 && kind != MODE_ACCUMULATE), "linear_int8: unknown element type %d of out for mode %d", out_dtype, mode);
     XRT_REQUIRE(((uintptr_t)a | (uintptr_t)w | (uintptr_t)w_scales) % 16 == 0, "linear_int8: rows, weights and their scales start at multiples of 16 bytes");
     if (M == 0) return 0;
+    XRT_REQUIRE(sizes_fit(M, N, mode), "linear_int8: too many rows, %d of a and %d of w", M, N);
     const long groups = int8_groups(N, kind == MODE_GATED);
     const Plan plan = plan_of(M, groups, int8_stride(K));
     const long need = sums_bytes(plan, M, groups);
     XRT_REQUIRE(need == 0 || (workspace && workspace_bytes >= need && (uintptr_t)workspace % 16 == 0), "linear_int8: a workspace of %ld bytes is needed, %ld given", need, workspace ? workspace_bytes : 0);
-    XRT_REQUIRE((long)M + 256 < (1L << 31) && groups * 16 < (1L << 30), "linear_int8: too many rows, %d of a and %d of w", M, N);
     const Operands o{(const signed char*)a, (const signed char*)w, (int4v*)workspace, (int)int8_stride(K), (int)groups, (hipStream_t)stream};
     if (out_dtype == XRT_BF16) {
         const Result<bf16> to{a_scales, w_scales, (bf16*)out, M, N, activation_of(mode)};

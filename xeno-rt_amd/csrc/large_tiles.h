@@ -45,8 +45,8 @@ inline long part_ids(long tiles, int parts, bool by_parts) { return by_parts ? (
 
 // The rows of a of each tile, where tiles of up to `most` rows (a multiple of 16) share M.
 inline int even_height(int M, int most) {
-    const int tiles = (M + most - 1) / most;
-    return ((M + tiles - 1) / tiles + 15) / 16 * 16;
+    const long tiles = ((long)M + most - 1) / most;
+    return (int)((M + tiles - 1) / tiles + 15) / 16 * 16;
 }
 
 // ---- the large tiles' small pieces
