@@ -96,3 +96,12 @@ def test_more_rows_than_32_bits_number_are_refused(lib):
     for m, n, mode in ((2 ** 31 - 1, 1, "store"), (2 ** 31 - 256, 1, "add"), (1, 2 ** 30, "store"), (1, 2 ** 29, "gated"), (4096, 2 ** 31 - 1, "store")):
         assert lib.xrt_linear_int8_plan(m, n, 64, MODES[mode], plan) != 0 and lib.xrt_linear_int8_workspace(m, n, 64, MODES[mode]) == 0
         assert lib.xrt_linear_int8(at, at, at, at, at, 0, m, n, 64, MODES[mode], None, ctypes.c_long(0), None) != 0 and b"too many rows" in lib.xrt_last_error()
+
+
+def test_more_threads_than_a_launch_counts_are_refused(lib):
+    lib.xrt_last_error.restype = ctypes.c_char_p
+    at = ctypes.c_void_p(1 << 20)
+    for m, n, mode in ((1, 2 ** 27 + 16, "store"), (1, 2 ** 29 - 64, "add"), (16, 2 ** 26 + 64, "gated"), (2 ** 31 - 300, 1, "store")):
+        assert lib.xrt_linear_int8(at, at, at, at, at, 0, m, n, 64, MODES[mode], None, ctypes.c_long(0), None) != 0
+        assert b"too many tiles" in lib.xrt_last_error(), (m, n, mode)
+    assert lib.xrt_pack_int8(at, at, at, at, 2 ** 29, 128, 0, None) != 0 and b"too many elements" in lib.xrt_last_error()

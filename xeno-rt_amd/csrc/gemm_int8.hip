@@ -572,7 +572,7 @@ template <int MT, int G, int MODE, typename TO, bool ONCE = true, bool SPLITS = 
 int launch_few(const Operands& o, const Plan& plan, const Result<TO>& to) {
     const int tiles_m = (to.M + MT * 16 - 1) / (MT * 16), tiles_n = (o.groups + G - 1) / G;
     const long ids = part_ids((long)tiles_m * tiles_n, plan.parts, true);        // a whole number of rounds over the XCDs
-    XRT_REQUIRE(ids < (1L << 31), "linear_int8: %ld tiles", ids);
+    XRT_REQUIRE(ids * WAVES * XRT_WAVE < XRT_INT8_GRID_THREADS, "linear_int8: too many tiles, %ld", ids);
     if (plan.parts == 1) gemm_int8_few_kernel<MT, G, MODE, TO, false, ONCE><<<(unsigned)ids, WAVES * XRT_WAVE, 0, o.stream>>>(o.a, o.w, nullptr, to.M, o.stride, o.groups, tiles_m, tiles_n, 1, to);
     else if constexpr (SPLITS) gemm_int8_few_kernel<MT, G, MODE_STORE, float, true, ONCE><<<(unsigned)ids, WAVES * XRT_WAVE, 0, o.stream>>>(o.a, o.w, o.sums, to.M, o.stride, o.groups, tiles_m, tiles_n, plan.parts, Result<float>{});
     XRT_REQUIRE(SPLITS || plan.parts == 1, "linear_int8: a product that is not cut, in %d parts", plan.parts);
@@ -583,6 +583,10 @@ template <int BM, int BN, int MODE, typename TO, bool PARTS>
 int launch_large(const Operands& o, const Plan& plan, const Result<TO>& to) {
     constexpr size_t lds = (size_t)2 * (BM + BN) * XRT_INT8_STEP + 2 * 256 * sizeof(float);
     auto kernel = gemm_int8_large_kernel<BM, BN, MODE, TO, PARTS>;
+    const int units = o.stride / XRT_INT8_STEP, steps = (units + plan.parts - 1) / plan.parts;
+    const int height = even_height(to.M, BM), tiles_m = (to.M + height - 1) / height, tiles_n = (o.groups + BN / 16 - 1) / (BN / 16);
+    const long ids = part_ids((long)tiles_m * tiles_n, plan.parts, true);        // a whole number of rounds over the XCDs
+    XRT_REQUIRE(ids * WAVES * XRT_WAVE < XRT_INT8_GRID_THREADS, "linear_int8: too many tiles, %ld", ids);
     static bool configured[64] = {};                           // per instantiation and device
     int device = 0;
     XRT_REQUIRE(hipGetDevice(&device) == hipSuccess, "linear_int8: no current device");
@@ -591,10 +595,6 @@ int launch_large(const Operands& o, const Plan& plan, const Result<TO>& to) {
         XRT_REQUIRE(e == hipSuccess, "linear_int8: cannot reserve %zu bytes of LDS: %s", lds, hipGetErrorString(e));
         if (device >= 0 && device < 64) configured[device] = true;
     }
-    const int units = o.stride / XRT_INT8_STEP, steps = (units + plan.parts - 1) / plan.parts;
-    const int height = even_height(to.M, BM), tiles_m = (to.M + height - 1) / height, tiles_n = (o.groups + BN / 16 - 1) / (BN / 16);
-    const long ids = part_ids((long)tiles_m * tiles_n, plan.parts, true);        // a whole number of rounds over the XCDs
-    XRT_REQUIRE(ids < (1L << 31), "linear_int8: %ld tiles", ids);
     kernel<<<(unsigned)ids, 8 * XRT_WAVE, lds, o.stream>>>(o.a, o.w, o.sums, o.stride, o.groups, tiles_m, tiles_n, height, plan.parts, steps, to);
     return 0;
 }

@@ -15,6 +15,8 @@
 #define XRT_INT8_STEP 128                   // columns that a product takes at a time
 #define XRT_INT8_MOST_K XRT_INT8_K_LIMIT    // 2^14 * k stays below 2^31: a sum of k products of two signed bytes fits 32 bits
 
+#define XRT_INT8_GRID_THREADS (1L << 32)    // a launch takes the number of its threads modulo this, without an error: there are fewer
+
 __host__ __device__ inline long int8_stride(long k) { return (k + XRT_INT8_STEP - 1) / XRT_INT8_STEP * XRT_INT8_STEP; }
 // groups of 16 packed rows of a matrix with n outputs
 __host__ __device__ inline long int8_groups(long n, bool gated) { return gated ? (n + 7) / 8 : (n + 15) / 16; }

@@ -5,6 +5,8 @@
 //
 // in float32, the division the exact one: a value next to a border between two integers falls to the side where float32 arithmetic written down plainly has
 // it. A row of zeros has scale 0. A row that holds an infinity or a NaN has scale NaN and zeros for values, so that whatever is made of it is NaN.
+#include <algorithm>
+
 #include "int8.h"
 #include "xrt_hip.h"
 
@@ -233,6 +235,13 @@ __global__ void __launch_bounds__(256) int8_pack_kernel(const signed char* __res
 // Threads of a row's workgroup, where each keeps up to `most` pieces.
 int threads_for(int stride, int most) { return whole_wavefronts(min(MOST_THREADS, (stride / 8 + most - 1) / most)); }
 
+// Calls launch(first, count) for runs of rows whose workgroups of `threads` threads (of `together` rows each) fit a launch.
+template <typename Launch>
+void in_runs(int rows, int threads, int together, Launch launch) {
+    const long most = (XRT_INT8_GRID_THREADS - 1) / threads * together;
+    for (long first = 0; first < rows; first += most) launch(first, (int)std::min(most, rows - first));
+}
+
 }  // namespace
 
 extern "C" long xrt_int8_stride(int k) { return int8_stride(k); }
@@ -246,7 +255,11 @@ extern "C" int xrt_quantize_int8(const void* x, int dtype, long x_stride, void* 
     if (rows == 0) return 0;
     const int stride = (int)int8_stride(k);
     hipStream_t s = (hipStream_t)stream;
-#define XRT_ROWS8(TX, PIECES) int8_rows_kernel<TX, float, float, false, PIECES><<<rows, threads_for(stride, PIECES), 0, s>>>((TX*)x, nullptr, nullptr, nullptr, (signed char*)values, scales, x_stride, rows, k, stride, 0.f)
+#define XRT_ROWS8(TX, PIECES)                                                                                                                            \
+    in_runs(rows, threads_for(stride, PIECES), 1, [&](long first, int count) {                                                                            \
+        int8_rows_kernel<TX, float, float, false, PIECES><<<count, threads_for(stride, PIECES), 0, s>>>(                                                  \
+            (TX*)x + first * x_stride, nullptr, nullptr, nullptr, (signed char*)values + first * stride, scales + first, x_stride, count, k, stride, 0.f); \
+    })
     // two pieces a thread up to 8192 columns, four beyond: more of a wide row is then in flight (bfloat16, 8192 rows of 14336: 104 us with one, 78 with two,
     // 67 with four, 73 with eight; 2048 of 8192: 19.0, 11.1, 11.8 and 11.6; 8192 of 513: 8.9, 5.9, 7.0 and 10.4)
     if (dtype == XRT_F32 && stride <= 8192) XRT_ROWS8(float, 2);
@@ -270,7 +283,12 @@ extern "C" int xrt_rmsnorm_int8(float* x, const void* delta, int delta_dtype, co
     if (n_rows == 0) return 0;
     const int stride = (int)int8_stride(hidden);
     hipStream_t s = (hipStream_t)stream;
-#define XRT_NORM8(TD, TW, PIECES) int8_rows_kernel<float, TD, TW, true, PIECES><<<n_rows, threads_for(stride, PIECES), 0, s>>>(x, (const TD*)delta, (const TW*)weight, rows, (signed char*)values, scales, hidden, x_rows, hidden, stride, eps)
+#define XRT_NORM8(TD, TW, PIECES)                                                                                                                           \
+    in_runs(n_rows, threads_for(stride, PIECES), 1, [&](long first, int count) {                                                                            \
+        int8_rows_kernel<float, TD, TW, true, PIECES><<<count, threads_for(stride, PIECES), 0, s>>>(                                                        \
+            rows ? x : x + first * hidden, delta ? (const TD*)delta + first * hidden : nullptr, (const TW*)weight, rows ? rows + first : nullptr,           \
+            (signed char*)values + first * stride, scales + first, hidden, rows ? x_rows : count, hidden, stride, eps);                                     \
+    })
 #define XRT_NORM8_OF(PIECES)                                                                      \
     do {                                                                                          \
         if (delta_dtype == XRT_BF16 && weight_dtype == XRT_BF16) XRT_NORM8(bf16, bf16, PIECES);   \
@@ -295,11 +313,16 @@ extern "C" int xrt_dequantize_int8(const void* values, const float* scales, void
     if (rows == 0) return 0;
     int lanes = 8;
     while (lanes < 256 && lanes * 8 < k) lanes *= 2;
-    const long chunks = (k + lanes * 8 - 1) / (lanes * 8), blocks = (rows + (long)(256 / lanes) - 1) / (256 / lanes) * chunks;
-    XRT_REQUIRE(blocks < (1L << 31), "dequantize_int8: too many elements");
+    const int chunks = (k + lanes * 8 - 1) / (lanes * 8), together = 256 / lanes, stride = (int)int8_stride(k);
     hipStream_t s = (hipStream_t)stream;
-    if (out_dtype == XRT_F32) int8_values_kernel<float><<<(unsigned)blocks, 256, 0, s>>>((const signed char*)values, scales, (float*)out, rows, k, (int)int8_stride(k), lanes, (unsigned)chunks);
-    else int8_values_kernel<bf16><<<(unsigned)blocks, 256, 0, s>>>((const signed char*)values, scales, (bf16*)out, rows, k, (int)int8_stride(k), lanes, (unsigned)chunks);
+#define XRT_VALUES8(TO)                                                                                                                                    \
+    in_runs(rows, 256 * chunks, together, [&](long first, int count) {                                                                                     \
+        int8_values_kernel<TO><<<(unsigned)((count + together - 1) / together * (long)chunks), 256, 0, s>>>(                                               \
+            (const signed char*)values + first * stride, scales + first, (TO*)out + first * k, count, k, stride, lanes, (unsigned)chunks);                 \
+    })
+    if (out_dtype == XRT_F32) XRT_VALUES8(float);
+    else XRT_VALUES8(bf16);
+#undef XRT_VALUES8
     XRT_LAUNCH_CHECK("dequantize_int8");
     return 0;
 }
@@ -309,7 +332,7 @@ extern "C" int xrt_pack_int8(const void* values, const float* scales, void* pack
     XRT_REQUIRE(((uintptr_t)values | (uintptr_t)packed) % 16 == 0, "pack_int8: values start at a multiple of 16 bytes");
     const long pieces = int8_groups(n, gated != 0) * int8_stride(k);             // 16 rows of stride bytes, 16 bytes a piece
     const long blocks = (pieces + 255) / 256;
-    XRT_REQUIRE(blocks < (1L << 31), "pack_int8: too many elements");
+    XRT_REQUIRE(blocks * 256 < XRT_INT8_GRID_THREADS, "pack_int8: too many elements, %d rows of %d columns", n, k);
     int8_pack_kernel<<<(unsigned)blocks, 256, 0, (hipStream_t)stream>>>((const signed char*)values, scales, (signed char*)packed, packed_scales, n, k,
                                                                         (int)int8_stride(k), pieces, gated != 0);
     XRT_LAUNCH_CHECK("pack_int8");
