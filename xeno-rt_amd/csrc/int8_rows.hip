@@ -104,7 +104,7 @@ __global__ void __launch_bounds__(MOST_THREADS) int8_rows_kernel(TX* x, const TD
                                                                  signed char* __restrict__ values, float* __restrict__ scales, long x_stride,
                                                                  int x_rows, int width, int stride, float eps) {
     __shared__ float sums[32];
-    __shared__ unsigned maxima[16];
+    __shared__ unsigned maxima[2][16];
     const long r = blockIdx.x;
     const long source = rows ? rows[r] : r;
     signed char* out = values + r * stride;
@@ -118,7 +118,7 @@ __global__ void __launch_bounds__(MOST_THREADS) int8_rows_kernel(TX* x, const TD
     const int step = blockDim.x * 8, first = threadIdx.x * 8;
     constexpr bool EARLY = NORM && PIECES <= 2;                 // the gains are asked for now, so that they arrive under the sum
     float kept[PIECES][8], gains[EARLY ? PIECES : 1][8];
-    float inv_rms = 1.f;
+    float inv_rms = 1.f, power = 1.f;                           // (power: of two, that the row is multiplied by where its squares do not fit float32)
 #pragma unroll
     for (int i = 0; i < PIECES; ++i) load_eight(row, first + i * step, width, kept[i]);
     if constexpr (EARLY)
@@ -147,7 +147,41 @@ __global__ void __launch_bounds__(MOST_THREADS) int8_rows_kernel(TX* x, const TD
 #pragma unroll
             for (int e = 0; e < 8; ++e) sum = fmaf(v[e], v[e], sum);
         }
-        inv_rms = 1.0f / sqrtf(block_sum(sum, sums) / (float)width + eps);
+        sum = block_sum(sum, sums);
+        const float mean = sum / (float)width + eps;
+        inv_rms = 1.0f / sqrtf(mean);
+        if (__builtin_expect(!(sum < __builtin_inff()) || mean < 0x1p-100f, 0)) {      // (the same for all threads)
+            // The squares overflow (elements of 2^64 / sqrt(width) and more) or vanish (eps is next to nothing). Of finite elements that are not all zero they are summed
+            // again, of the row times a power of two: the quotient does not change by it.
+            unsigned largest = 0u;
+            auto each = [&](auto look) {                        // (the thread's elements that are not kept, as they lie in memory)
+                for (int at = first + PIECES * step; at < width; at += step) {
+                    float v[8];
+                    load_eight(row, at, width, v);
+#pragma unroll
+                    for (int e = 0; e < 8; ++e) look(v[e]);
+                }
+            };
+#pragma unroll
+            for (int i = 0; i < PIECES; ++i)
+#pragma unroll
+                for (int e = 0; e < 8; ++e) largest = max(largest, magnitude_bits(kept[i][e]));
+            each([&](float v) { largest = max(largest, magnitude_bits(v)); });
+            largest = block_max_bits(largest, maxima[1]);
+            if (largest > 0u && largest < 0x7f800000u) {
+                power = sum < 1.f ? 0x1p100f : 0x1p-80f;
+                sum = 0.f;
+#pragma unroll
+                for (int i = 0; i < PIECES; ++i)
+#pragma unroll
+                    for (int e = 0; e < 8; ++e) {
+                        kept[i][e] *= power;
+                        sum = fmaf(kept[i][e], kept[i][e], sum);
+                    }
+                each([&](float v) { sum = fmaf(v * power, v * power, sum); });
+                inv_rms = 1.0f / sqrtf(block_sum(sum, sums) / (float)width + eps * power * power);
+            }
+        }
     }
     // what is brought to 8 bits, of what the row holds (a thread reads again only what it wrote itself)
     auto times = [&](float (&v)[8], const float (&gain)[8]) {
@@ -161,6 +195,12 @@ __global__ void __launch_bounds__(MOST_THREADS) int8_rows_kernel(TX* x, const TD
             times(v, gain);
         }
     };
+    auto finished_again = [&](int at, float (&v)[8]) {          // the same of a row read again, which lies in memory as it was
+        if constexpr (NORM)
+#pragma unroll
+            for (int e = 0; e < 8; ++e) v[e] *= power;
+        finished(at, v);
+    };
     unsigned most = 0u;
 #pragma unroll
     for (int i = 0; i < PIECES; ++i) {
@@ -172,18 +212,18 @@ __global__ void __launch_bounds__(MOST_THREADS) int8_rows_kernel(TX* x, const TD
     for (int at = first + PIECES * step; at < width; at += step) {
         float v[8];
         load_eight(row, at, width, v);
-        finished(at, v);
+        finished_again(at, v);
 #pragma unroll
         for (int e = 0; e < 8; ++e) most = max(most, magnitude_bits(v[e]));
     }
-    const float scale = scale_of(block_max_bits(most, maxima));
+    const float scale = scale_of(block_max_bits(most, maxima[0]));
 #pragma unroll
     for (int i = 0; i < PIECES; ++i)
         if (first + i * step < stride) *reinterpret_cast<uint2*>(out + first + i * step) = eight_bytes(kept[i], scale);
     for (int at = first + PIECES * step; at < stride; at += step) {
         float v[8];
         load_eight(row, at, width, v);
-        finished(at, v);
+        finished_again(at, v);
         *reinterpret_cast<uint2*>(out + at) = eight_bytes(v, scale);
     }
     if (threadIdx.x == 0) scales[r] = scale;

@@ -115,8 +115,8 @@ long xrt_int8_stride(int k);
 // scales[m] = max |x[m]| / 127, values = x / scale rounded to the nearest integer, halves to even; x (float32 or bfloat16) has its rows x_stride
 // elements apart. A row of zeros: scale 0; one with an infinity or a NaN: scale NaN and zeros.
 int xrt_quantize_int8(const void* x, int dtype, long x_stride, void* values, float* scales, int rows, int k, void* stream);
-// x[m] += delta[m] (delta may be null), then the rows rmsnorm(x[rows ? rows[r] : r]) * weight likewise; delta and rows not both. x has x_rows rows; an
-// index that is none of them gives zeros with scale NaN.
+// x[m] += delta[m] (delta may be null), then the rows x / sqrt(mean(x^2) + eps) * weight of x[rows ? rows[r] : r] likewise, also where the squares of a finite
+// row do not fit float32; delta and rows not both. x has x_rows rows; an index that is none of them gives zeros with scale NaN.
 int xrt_rmsnorm_int8(float* x, const void* delta, int delta_dtype, const void* weight, int weight_dtype, float eps, void* values, float* scales,
                      const int* rows, int n_rows, int x_rows, int hidden, void* stream);
 // out[m][j] = values[m][j] * scales[m]

@@ -662,8 +662,8 @@ class HipOps:
 
     def rmsnorm_int8(self, x, weight, eps, out: Int8Rows, delta=None, rows=None):
         """x += delta in place, if given (float32 or bfloat16, shaped like x), then out = the rows x / sqrt(mean(x^2) + eps) * weight as `quantize_int8`
-        would make them of float32. x is float32. rows: the rows of x that are wanted, as in `rmsnorm` (not together with delta); one that x does not
-        have gives zeros with scale NaN."""
+        would make them of float32, also of rows whose squares do not fit float32. x is float32. rows: the rows of x that are wanted, as in `rmsnorm` (not
+        together with delta); one that x does not have gives zeros with scale NaN."""
         if not isinstance(out, Int8Rows):
             raise KernelError("rmsnorm_int8 out: expected Int8Rows")
         (count, hidden), index = out.shape, out.index
