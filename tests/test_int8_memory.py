@@ -1,4 +1,4 @@
-"""Memory of the operators on 8-bit rows while a step of an engine runs, without a GPU: the checks of devices are taken out, the library is a stand-in that
+"""What the operators on 8-bit rows keep, and their memory while a step of an engine runs, without a GPU: the checks of devices are taken out, the library is a stand-in that
 keeps the addresses it is given."""
 import pytest
 import torch
@@ -66,3 +66,17 @@ def test_a_products_workspace_is_not_the_steps_memory(ops):
     with runtime.step_memory():
         ops.linear_int8(a, w, torch.zeros(4, 20))
         assert ops.lib.workspace and not inside(runtime, ops.lib.workspace)
+
+
+def test_what_was_checked_stays_what_it_is(ops):
+    """The calls take sizes from the rows and the matrix: larger ones, written over them, would be read behind the end of their tensors."""
+    a = hip.Int8Rows(torch.zeros(4, 128, dtype=torch.int8), torch.zeros(4), 100)
+    w = hip.Int8Matrix(torch.zeros(32, 128, dtype=torch.int8), torch.zeros(32), 20, 100, False)
+    before = a.shape, a.k, a.index, w.shape, w.gated, w.index
+    for made, names in ((a, ("shape", "index", "values", "scales", "k", "_values", "_scales", "_k", "other")), (w, ("shape", "gated", "index", "data", "scales", "_data", "_scales"))):
+        for name in names:
+            with pytest.raises(AttributeError):
+                setattr(made, name, (8, 100))
+            with pytest.raises(AttributeError):
+                delattr(made, name)
+    assert (a.shape, a.k, a.index, w.shape, w.gated, w.index) == before

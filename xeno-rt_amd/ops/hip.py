@@ -114,7 +114,23 @@ INT8_STEP = 128             # columns that a row of 8-bit values is filled up to
 INT8_MOST_K = 131071        # columns of which a sum of products still fits 32 bits (XRT_INT8_MOST_K)
 
 
-class Int8Rows:
+class _Checked:
+    """What is checked when it is made, and not again by the calls that take it, stays what it is."""
+
+    __slots__ = ()
+
+    def _keep(self, **fields) -> None:
+        for name, value in fields.items():
+            object.__setattr__(self, name, value)
+
+    def __setattr__(self, name, value):
+        raise AttributeError(f"{type(self).__name__}.{name} was checked when it was made and cannot be changed: make another one")
+
+    def __delattr__(self, name):
+        self.__setattr__(name, None)
+
+
+class Int8Rows(_Checked):
     """Rows in 8-bit integers: row m stands for values[m, :k] * scales[m]. values is int8 [rows, k filled up to a multiple of INT8_STEP] (what lies behind the
     k columns does not count), scales float32 [rows]. `int8_rows` makes an empty one; `quantize_int8` and `rmsnorm_int8` fill it, `linear_int8` and
     `linear_glu_int8` multiply it. The tensors are checked here, once, and stay what they are."""
@@ -129,7 +145,7 @@ class Int8Rows:
         HipOps._require(scales, "scales of 8-bit rows", torch.float32, (rows,), values)
         if values.data_ptr() % 16 != 0:                         # (they are read sixteen bytes at a time)
             raise KernelError("8-bit values must start at a multiple of 16 bytes")
-        self._values, self._scales, self._k, self.shape, self.index = values, scales, k, (rows, k), values.get_device()
+        self._keep(_values=values, _scales=scales, _k=k, shape=(rows, k), index=values.get_device())
 
     @property
     def values(self) -> torch.Tensor:
@@ -148,7 +164,7 @@ class Int8Rows:
         return self._values.device
 
 
-class Int8Matrix:
+class Int8Matrix(_Checked):
     """A weight matrix [rows, k] in 8-bit integers with a scale for each row (output channel), in the tiles in which the products take it
     (csrc/int8.h). gated: [gate rows | up rows], for `linear_glu_int8`. Made by `pack_int8`. The tensors are checked here, once, and stay what they are."""
 
@@ -163,7 +179,7 @@ class Int8Matrix:
         HipOps._require(scales, "scales of 8-bit weights", torch.float32, (packed_rows,), data)
         if data.data_ptr() % 16 != 0 or scales.data_ptr() % 16 != 0:
             raise KernelError("8-bit weights and their scales must start at multiples of 16 bytes")
-        self._data, self._scales, self.shape, self.gated, self.index = data, scales, (int(rows), int(k)), bool(gated), data.get_device()
+        self._keep(_data=data, _scales=scales, shape=(int(rows), int(k)), gated=bool(gated), index=data.get_device())
 
     @property
     def data(self) -> torch.Tensor:
