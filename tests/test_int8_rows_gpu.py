@@ -73,3 +73,10 @@ def test_norm_of_huge_rows_that_hold_an_infinity_or_a_nan(ops):
         ops.rmsnorm_int8(x, torch.ones(300, device=DEV), eps, out)
         assert bool(torch.isnan(out.scales[1:3]).all()) and not out.values[1:].any() and bool(out.scales[0] > 0)
         assert bool(out.scales[3] == 0) if eps > 0 else bool(torch.isnan(out.scales[3]))      # (without an eps: zero by zero)
+
+
+def test_norm_of_rows_chosen_of_none(ops):
+    x, out = rand(0, 300), ops.int8_rows(3, 300, DEV)
+    out.values.fill_(55)
+    ops.rmsnorm_int8(x, torch.ones(300, device=DEV), EPS, out, rows=torch.tensor([0, -1, 7], dtype=torch.int32, device=DEV))
+    assert bool(torch.isnan(out.scales).all()) and not out.values.any()

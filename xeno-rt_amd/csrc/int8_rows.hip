@@ -313,7 +313,7 @@ extern "C" int xrt_quantize_int8(const void* x, int dtype, long x_stride, void* 
 
 extern "C" int xrt_rmsnorm_int8(float* x, const void* delta, int delta_dtype, const void* weight, int weight_dtype, float eps, void* values, float* scales,
                                 const int* rows, int n_rows, int x_rows, int hidden, void* stream) {
-    XRT_REQUIRE(n_rows >= 0 && x_rows >= 0 && hidden > 0 && hidden <= XRT_INT8_MOST_K && (n_rows == 0 || (x && weight && values && scales)),
+    XRT_REQUIRE(n_rows >= 0 && x_rows >= 0 && hidden > 0 && hidden <= XRT_INT8_MOST_K && (n_rows == 0 || ((x || x_rows == 0) && weight && values && scales)),
                 "rmsnorm_int8: bad operands rows=%d hidden=%d", n_rows, hidden);
     XRT_REQUIRE((weight_dtype == XRT_F32 || weight_dtype == XRT_BF16) && (!delta || delta_dtype == XRT_F32 || delta_dtype == XRT_BF16),
                 "rmsnorm_int8: unknown dtype weight=%d delta=%d", weight_dtype, delta_dtype);
