@@ -1,5 +1,8 @@
 """What the operators on 8-bit rows keep, and their memory while a step of an engine runs, without a GPU: the checks of devices are taken out, the library is a stand-in that
 keeps the addresses it is given."""
+import copy
+import pickle
+
 import pytest
 import torch
 
@@ -80,3 +83,13 @@ def test_what_was_checked_stays_what_it_is(ops):
             with pytest.raises(AttributeError):
                 delattr(made, name)
     assert (a.shape, a.k, a.index, w.shape, w.gated, w.index) == before
+
+
+def test_rows_and_matrices_can_be_copied_and_kept_in_files(ops):
+    a = hip.Int8Rows(torch.arange(512).to(torch.int8).view(4, 128), torch.rand(4), 100)
+    w = hip.Int8Matrix(torch.ones(32, 128, dtype=torch.int8), torch.rand(32), 40, 100, True)
+    for copied in (copy.copy, copy.deepcopy, lambda made: pickle.loads(pickle.dumps(made))):
+        b, v = copied(a), copied(w)
+        assert torch.equal(b.values, a.values) and torch.equal(b.scales, a.scales) and (b.shape, b.k, b.index) == (a.shape, a.k, a.index)
+        assert torch.equal(v.data, w.data) and torch.equal(v.scales, w.scales) and (v.shape, v.gated, v.index) == (w.shape, w.gated, w.index)
+    assert copy.deepcopy(a).values.data_ptr() != a.values.data_ptr()

@@ -115,7 +115,7 @@ INT8_MOST_K = 131071        # columns of which a sum of products still fits 32 b
 
 
 class _Checked:
-    """What is checked when it is made, and not again by the calls that take it, stays what it is."""
+    """What is checked when it is made, and not again by the calls that take it, stays what it is. A copy, or one read from a file, is made and checked anew."""
 
     __slots__ = ()
 
@@ -146,6 +146,9 @@ class Int8Rows(_Checked):
         if values.data_ptr() % 16 != 0:                         # (they are read sixteen bytes at a time)
             raise KernelError("8-bit values must start at a multiple of 16 bytes")
         self._keep(_values=values, _scales=scales, _k=k, shape=(rows, k), index=values.get_device())
+
+    def __reduce__(self):
+        return Int8Rows, (self._values, self._scales, self._k)
 
     @property
     def values(self) -> torch.Tensor:
@@ -180,6 +183,9 @@ class Int8Matrix(_Checked):
         if data.data_ptr() % 16 != 0 or scales.data_ptr() % 16 != 0:
             raise KernelError("8-bit weights and their scales must start at multiples of 16 bytes")
         self._keep(_data=data, _scales=scales, shape=(int(rows), int(k)), gated=bool(gated), index=data.get_device())
+
+    def __reduce__(self):
+        return Int8Matrix, (self._data, self._scales, *self.shape, self.gated)
 
     @property
     def data(self) -> torch.Tensor:
