@@ -131,15 +131,15 @@ constexpr int WAVES = 8;
 // MT: blocks of 16 rows of a; G: groups of 16 packed rows of w a workgroup. Its wavefronts share out k, each with a run of its own, and add their sums
 // through LDS. Nothing is read twice by a workgroup, so a's rows come from L2 as often as there are workgroups along n: with G groups a workgroup reads
 // MT / G times as much of a as of w. PARTS: k is cut among workgroups. ONCE: the rows of a are one tile, so that every byte of w is read by one workgroup,
-// and is asked for past the caches. Reading w bounds it: 8 rows, k = 4096, 14336 pairs 18.6 us, 6.3 TB/s; 128256 channels 76 us, 6.9 TB/s; a kernel that only reads 7.2.
+// and is asked for past the caches. Reading w bounds it: 8 rows, k = 4096, 14336 pairs 19.5 us, 6.0 TB/s; 128256 channels 83 us, 6.4 TB/s; a kernel that only reads 7.2.
 template <int MT, int G, int MODE, typename TO, bool PARTS, bool ONCE>
 __global__ void __launch_bounds__(WAVES * XRT_WAVE, MT * G <= 2 ? 4 : 2) gemm_int8_few_kernel(const signed char* __restrict__ a, const signed char* __restrict__ w,
                                                                                           int4v* __restrict__ sums, int M, int stride, int groups, int tiles_m,
                                                                                           int tiles_n, int parts, const Result<TO> to) {
     constexpr int AT_ONCE = G * MT < 8 ? G * MT : 8;            // blocks whose sums lie in LDS at one time
     __shared__ int4v shared[WAVES][AT_ONCE][XRT_WAVE];
-    // An XCD gets a run of tiles; split over one tile of rows: tiles and parts in turn. (8 rows, k = 4096, 1792 groups 20.4 us in runs, 23.2 in turn; 64 rows,
-    // k = 14336, 4096 channels in four parts 19.4 and 17.8.)
+    // An XCD gets a run of tiles; split over one tile of rows: tiles and parts in turn. (33 rows, k = 4096, 1792 groups 26.0 us in runs, 28.6 in turn, 8 rows 19.5 either way;
+    // 64 rows, k = 14336, 4096 channels in four parts 19.2 and 17.9.)
     const PartPlace place = few_place(blockIdx.x, tiles_m, tiles_n, PARTS, parts, ONCE);
     if (place.tile.m < 0) return;
     const int lane = threadIdx.x % XRT_WAVE, wave = __builtin_amdgcn_readfirstlane(threadIdx.x / XRT_WAVE);
@@ -184,8 +184,8 @@ __global__ void __launch_bounds__(WAVES * XRT_WAVE, MT * G <= 2 ? 4 : 2) gemm_in
 #pragma unroll
                 for (int i = 0; i < MT; ++i) acc[g][i] = __builtin_amdgcn_mfma_i32_16x16x64_i8(unit.w[g][j], unit.a[i][j], acc[g][i], 0, 0, 0);
     };
-    // Two units in turn: while one is multiplied the other is on its way. (Three or four cost the workgroups that run beside this one their registers:
-    // 32 rows, k = 4096, 14336 pairs 30.1 us with three, 27.7 with two.)
+    // Two units in turn: while one is multiplied the other is on its way. (Three cost the workgroups that run beside this one their registers: 32 rows, k = 4096,
+    // 14336 pairs 25.2 us with three, 23.1 with two; 64 rows, which then spill, 66.8 and 31.0.)
     constexpr int RING = 2;
     Unit ring[RING];
 #pragma unroll
@@ -229,8 +229,8 @@ __global__ void __launch_bounds__(WAVES * XRT_WAVE, MT * G <= 2 ? 4 : 2) gemm_in
 // ---- more rows --------------------------------------------------------------------------------------------------------------------------------------------
 
 // Tiles of BM (256, 192 or 128) rows of a by BN (256, or 128) packed rows of w: eight wavefronts, two to a SIMD, which take turns as those of the bfloat16 product's
-// large tiles do. Power bounds it: 4096 rows, k = 14336, 8192 channels 310 us, 3.1 Pop/s, as much as these instructions reach on numbers that stay in registers; at
-// k = 4096, 14336 pairs 342 to 362 us, of which a round's first loads and its results take a sixth. Of the two on a SIMD (one of each group of four) one reads the operands of its next products from LDS and asks for tiles to come while the other
+// large tiles do. Power bounds it: 4096 rows, k = 14336, 8192 channels 310 to 329 us, 2.9 to 3.1 Pop/s; these instructions reach 3.1 on numbers that stay in registers; at
+// k = 4096, 14336 pairs 342 to 373 us, of which a round's first loads and its results take a sixth. Of the two on a SIMD (one of each group of four) one reads the operands of its next products from LDS and asks for tiles to come while the other
 // multiplies; a barrier ends a turn, and the second group runs one barrier behind the first. A wavefront's part (BM / 2 x BN / 4) is four quarters along k: (half
 // h of its rows of a, half g of its rows of w) in the order (0,0) (0,1) (1,1) (1,0), so that every turn reads one new half: w0, w1, a1, and a0 of the next
 // tile. A half is loaded into the place of the same half two tiles ago as soon as both groups have read that, seven quarters before it is needed, and the
@@ -530,7 +530,7 @@ Plan plan_of(long M, long groups, long stride) {
     // workgroups (us, and of the larger tiles: 217 rows, k = 384, 1312 channels 4.5 and 6.9; 1233, 5342, 497 15.7 and 17.9; 119, 5724, 4235 19.6 and 15.5; 225, 6021, 4037
     // 18.4 and 18.7; 92, 8327, 4784 23.4 and 16.4), else 32 a part (144, 15612, 928 14.1 and 15.4; 256, 13719, 1101 19.2 and 17.7; 480, 16494, 975 26.0 and 21.8).
     {
-        // (two blocks of rows, 1792 groups of w: 27.7 us with two groups a workgroup, 24.5 with four; 384 groups: 9.5 and 11.1)
+        // (two blocks of rows, 1792 groups of w: 26.8 us with two groups a workgroup, 23.0 with four; 384 groups: 8.6 and 10.7)
         Plan plan{0, 0, M <= 16 ? 1 : M <= 32 ? 2 : 4, M <= 16 ? 1 : M <= 32 && groups < 4 * XRT_COMPUTE_UNITS ? 2 : 4, 1};
         const long workgroups = (M + plan.blocks * 16 - 1) / (plan.blocks * 16) * ((groups + plan.groups - 1) / plan.groups);
         // k in as many parts as there are compute units for, each of 12 units of 128 columns by 16 rows at least, if the longest way along k gets shorter by 48 of them:

@@ -30,6 +30,8 @@ namespace {
 typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
 typedef float floatx16 __attribute__((ext_vector_type(16)));
 typedef float floatx4 __attribute__((ext_vector_type(4)));
+template <typename T> struct alignas(sizeof(T) * 4) Four { T e[4]; };
+
 constexpr int BK = 64;
 constexpr int PITCH = BK + 8;          // bf16 elements per LDS row
 enum { MODE_STORE = 0, MODE_ACCUMULATE = 1, MODE_GATED = 2 };
@@ -452,6 +454,36 @@ __device__ __forceinline__ void gemm_tile(
                     }
                 }
         }
+    }
+}
+
+// ---- the large tiles' small pieces (the others, which products of 8-bit rows share: large_tiles.h)
+// Four neighbouring columns of a row of out [M][N], in one piece where `wide` says that rows and columns allow it.
+template <typename TO>
+__device__ __forceinline__ void load_four(const TO* out, long m, long n, int M, int N, float (&v)[4], bool wide) {
+    const TO* row = out + min(m, (long)M - 1) * (long)N;       // (rows and columns beyond the matrix: something inside, not used)
+    if (wide) {
+        const Four<TO> four = *reinterpret_cast<const Four<TO>*>(row + min(n, (long)N - 4));
+#pragma unroll
+        for (int e = 0; e < 4; ++e) v[e] = to_float(four.e[e]);
+    } else {
+#pragma unroll
+        for (int e = 0; e < 4; ++e) v[e] = to_float(row[min(n + e, (long)N - 1)]);
+    }
+}
+template <typename TO>
+__device__ __forceinline__ void store_four(TO* out, long m, long n, int M, int N, const float (&v)[4], bool wide) {
+    if (m >= M || n >= N) return;
+    TO* row = out + m * (long)N;
+    if (wide) {
+        Four<TO> four;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) four.e[e] = from_float<TO>(v[e]);
+        *reinterpret_cast<Four<TO>*>(row + n) = four;
+    } else {
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+            if (n + e < N) row[n + e] = from_float<TO>(v[e]);
     }
 }
 

@@ -230,7 +230,7 @@ __global__ void __launch_bounds__(MOST_THREADS) int8_rows_kernel(TX* x, const TD
 }
 
 // out[m][j] = values[m][j] * scales[m]: `lanes` threads a row (a power of two up to 256), a thread eight neighbouring columns. (8192 rows of 14336 to
-// bfloat16 61 us, 5.8 TB/s; 8 rows of 4096 2.3 us, an empty kernel 2.)
+// bfloat16 63 us, 5.6 TB/s; 8 rows of 4096 2.3 us, an empty kernel 2.)
 template <typename TO>
 __global__ void __launch_bounds__(256) int8_values_kernel(const signed char* __restrict__ values, const float* __restrict__ scales, TO* __restrict__ out,
                                                           int rows, int width, int stride, int lanes, unsigned chunks) {
@@ -300,8 +300,9 @@ extern "C" int xrt_quantize_int8(const void* x, int dtype, long x_stride, void* 
         int8_rows_kernel<TX, float, float, false, PIECES><<<count, threads_for(stride, PIECES), 0, s>>>(                                                  \
             (TX*)x + first * x_stride, nullptr, nullptr, nullptr, (signed char*)values + first * stride, scales + first, x_stride, count, k, stride, 0.f); \
     })
-    // two pieces a thread up to 8192 columns, four beyond: more of a wide row is then in flight (bfloat16, 8192 rows of 14336: 104 us with one, 78 with two,
-    // 67 with four, 73 with eight; 2048 of 8192: 19.0, 11.1, 11.8 and 11.6; 8192 of 513: 8.9, 5.9, 7.0 and 10.4)
+    // two pieces a thread up to 8192 columns, four beyond: more of a wide row is then in flight (bfloat16, three matrices in turn, 8192 rows of 14336: 96 us with one, 70
+    // with two, 65 with four, 71 with eight; 33 of 25600: 7.0, 5.0, 4.5 and 5.1; 2048 of 8192: 18.1, 10.8, 11.4 and 11.3; 8192 of 513: 8.8, 5.8, 6.8 and 10.3. float32: 113, 102, 109 and
+    // 110; 6.5, 4.8, 4.4 and 4.6; 19.2, 13.9, 14.0 and 14.3; 9.0, 7.1, 8.0 and 11.3. Behind other kernels, which leave less of the last cache to it, the first takes 79 us, in float32 125.)
     if (dtype == XRT_F32 && stride <= 8192) XRT_ROWS8(float, 2);
     else if (dtype == XRT_F32) XRT_ROWS8(float, 4);
     else if (stride <= 8192) XRT_ROWS8(bf16, 2);
@@ -336,8 +337,8 @@ extern "C" int xrt_rmsnorm_int8(float* x, const void* delta, int delta_dtype, co
         else if (weight_dtype == XRT_BF16) XRT_NORM8(float, bf16, PIECES);                        \
         else XRT_NORM8(float, float, PIECES);                                                     \
     } while (0)
-    // two pieces a thread, with the gains in registers ahead of the sum (8 rows of 4096 4.4 us, 4.8 with one piece, 5.3 with four and the gains fetched behind
-    // the sum; 333 of 5120 7.9, 9.5 and 8.4; 16384 of 4096 the same with either: 150 us, 4.9 TB/s, the rate of a copy)
+    // two pieces a thread, with the gains in registers ahead of the sum (8 rows of 4096 4.3 us, 4.7 with one piece, 5.0 with four and the gains fetched behind
+    // the sum; 333 of 5120 7.2, 8.9 and 7.9; 1001 of 2049 8.1, 9.8 and 8.8; 16384 of 4096 148 us, 148 and 154: 5.0 TB/s, the rate of a copy)
     if (stride <= 2 * 8 * MOST_THREADS) XRT_NORM8_OF(2);
     else XRT_NORM8_OF(4);
 #undef XRT_NORM8_OF

@@ -7,8 +7,6 @@ namespace {
 
 typedef unsigned uint4v __attribute__((ext_vector_type(4)));
 
-template <typename T> struct alignas(sizeof(T) * 4) Four { T e[4]; };
-
 // Which tile of tiles_m x tiles_n a workgroup takes. Ids are dealt to the XCDs round-robin: each XCD gets a contiguous run of
 // tiles, and a run is walked n-fastest inside panels of 8 n-tiles, so that the tiles that run at one time on an XCD share a
 // and w in its L2; m-fastest where there are up to four rows of tiles (a panel's tiles of one n would often lie on two XCDs, which then both read their w), but not where k
@@ -80,34 +78,6 @@ __device__ __forceinline__ uint4v join_rows(const float (&first)[4], const float
     const auto low = __builtin_amdgcn_permlane16_swap(two_bf16<TO>(first[0], first[1]), two_bf16<TO>(second[0], second[1]), false, false);
     const auto high = __builtin_amdgcn_permlane16_swap(two_bf16<TO>(first[2], first[3]), two_bf16<TO>(second[2], second[3]), false, false);
     return uint4v{low[0], high[0], low[1], high[1]};
-}
-// Four neighbouring columns of a row of out [M][N], in one piece where `wide` says that rows and columns allow it.
-template <typename TO>
-__device__ __forceinline__ void load_four(const TO* out, long m, long n, int M, int N, float (&v)[4], bool wide) {
-    const TO* row = out + min(m, (long)M - 1) * (long)N;       // (rows and columns beyond the matrix: something inside, not used)
-    if (wide) {
-        const Four<TO> four = *reinterpret_cast<const Four<TO>*>(row + min(n, (long)N - 4));
-#pragma unroll
-        for (int e = 0; e < 4; ++e) v[e] = to_float(four.e[e]);
-    } else {
-#pragma unroll
-        for (int e = 0; e < 4; ++e) v[e] = to_float(row[min(n + e, (long)N - 1)]);
-    }
-}
-template <typename TO>
-__device__ __forceinline__ void store_four(TO* out, long m, long n, int M, int N, const float (&v)[4], bool wide) {
-    if (m >= M || n >= N) return;
-    TO* row = out + m * (long)N;
-    if (wide) {
-        Four<TO> four;
-#pragma unroll
-        for (int e = 0; e < 4; ++e) four.e[e] = from_float<TO>(v[e]);
-        *reinterpret_cast<Four<TO>*>(row + n) = four;
-    } else {
-#pragma unroll
-        for (int e = 0; e < 4; ++e)
-            if (n + e < N) row[n + e] = from_float<TO>(v[e]);
-    }
 }
 
 }  // namespace
