@@ -127,6 +127,7 @@ long xrt_int8_packed_rows(int n, int gated);
 int xrt_pack_int8(const void* values, const float* scales, void* packed, float* packed_scales, int n, int k, int gated, void* stream);
 // out[m][n] (+)= (sum_k a[m][k] * w[n][k]) * a_scales[m] * w_scales[n], modes as xrt_linear has them, w packed (mode 2: as a gated matrix); the sum is exact,
 // so the result of a row does not depend on the others. xrt_linear_int8_workspace: the bytes that a product split along k needs (0: none).
+// M up to 2^31 - 257 and packed rows below 2^30, as far as their tiles have threads in a launch; more is refused.
 int xrt_linear_int8(const void* a, const float* a_scales, const void* w, const float* w_scales, void* out, int out_dtype, int M, int N, int K,
                     int mode, void* workspace, long workspace_bytes, void* stream);
 long xrt_linear_int8_workspace(int M, int N, int K, int mode);
